@@ -53,6 +53,7 @@ typedef int32_t sfk_status;
 #define SFK_TYPE_Q4_K 12
 #define SFK_TYPE_Q6_K 14
 #define SFK_TYPE_Q8_K 15
+#define SFK_TYPE_BF16 30 /* activation rows of the paged-cache operators only */
 
 /* tensor ids (GGUF names used by engine.cpp:1854-1989,2712,2994) */
 #define SFK_T_TOK_EMBD 0       /* token_embd.weight          [d, V]        */
@@ -71,6 +72,7 @@ typedef int32_t sfk_status;
 
 #define SFK_KV_F32 0
 #define SFK_KV_F16 1
+#define SFK_KV_BF16 2 /* the paged-cache operators only */
 
 /* Model shape and engine options.  The first block mirrors
  * engine::EngineHParams (engine.h:41-55); types name the quantization of each
@@ -490,6 +492,90 @@ SFK_API sfk_status sfk_attn_decode_paged(const float *dev_q, const void *dev_k_p
                                  int32_t n_pages, const int32_t *dev_page_table, int32_t max_pages, const int32_t *dev_positions,
                                  int32_t b, int32_t n_head, int32_t n_head_kv, int32_t head_dim, float *dev_out,
                                  void *stream);
+
+/* ---- paged-cache operators (operator level; device pointers) -------------
+ * The engine's cache as three calls of their own: what writes it
+ * (sfk_qk_norm_rope_append) and what reads it, for one new token of each
+ * sequence (sfk_attn_decode_window) and for prompts (sfk_attn_prefill_window).
+ * Beyond the engine's own path they take 16-bit rows, any number of sequences,
+ * models that norm each head of q and k, half-split and partial rotations,
+ * positions of several axes, and attention through a sliding window.
+ *
+ * Common to the three:
+ *   - Cache: k_pages / v_pages [n_pages][n_head_kv][16][head_dim] of kv_type
+ *     (SFK_KV_F32 / _F16 / _BF16), 16-byte aligned; page_table [..][max_pages]
+ *     of page ids per sequence.  Entries of pages that a call neither writes
+ *     nor sees are never looked at.
+ *   - io_type: SFK_TYPE_F32 / _F16 / _BF16, the type of q, k, v, q_out and
+ *     out.  Strides count elements between tokens; a token's heads are
+ *     contiguous ([n_head][head_dim]), so q, k and v may be parts of one packed
+ *     row.
+ *   - A call launches on `stream` (of the current device, where the pointers
+ *     live) and returns without waiting.  It allocates nothing and keeps
+ *     nothing: calls on several streams are independent, and all three can be
+ *     captured into CUDA graphs.
+ *   - dev_status (optional): one device int32, zero before the first call.  A
+ *     position, length, sequence or page id outside its range is never
+ *     dereferenced; it stores a code there, and sfk_device_status (which waits
+ *     for the stream) turns the code into SFK_ERR_RUNTIME and clears the word.
+ */
+
+/* q, k (optionally) normed and rotated, q to q_out, k and v appended to the
+ * cache, all heads of n_tok tokens in one launch.
+ *   norm:     x * rsqrt(mean(x^2) + eps) * w over each head; q_norm / k_norm
+ *             [head_dim] f32, NULL: none.
+ *   rotation: the first n_rot dims of each head (0: none) in n_rot / 2 pairs,
+ *             pair i = (2i, 2i+1), or (i, i + n_rot/2) with neox; angle =
+ *             position * freqs[i], the product taken in 64 bits.  n_rot is a
+ *             multiple of 8, of 16 with neox; freqs [n_rot/2] f32 (device).
+ *   positions: rope_pos NULL: the cache position.  Otherwise rope_pos
+ *             [n_axes][n_tok] (device) and rope_axis [n_rot/2] (HOST, NULL:
+ *             all 0) names each pair's axis, e.g. time, height and width.
+ *   slot:     token t goes to position pos[t] of sequence seq[t] (seq NULL:
+ *             sequence t).  pos[t] < 0: a padding row, nothing of it is
+ *             written.  A slot is given at most once in a call.
+ * head_dim is a multiple of 8 up to 256; any io_type with any kv_type, rounded
+ * once.  q_out may be q itself (same stride). */
+SFK_API sfk_status sfk_qk_norm_rope_append(
+    int32_t io_type, const void *dev_q, int64_t q_stride, const void *dev_k, int64_t k_stride, const void *dev_v,
+    int64_t v_stride, int32_t n_tok, int32_t n_head, int32_t n_head_kv, int32_t head_dim, const float *dev_q_norm,
+    const float *dev_k_norm, float eps, int32_t neox, int32_t n_rot, const float *dev_freqs, const int32_t *dev_rope_pos,
+    int32_t n_axes, const uint8_t *rope_axis, int32_t kv_type, void *dev_k_pages, void *dev_v_pages, int32_t n_pages,
+    const int32_t *dev_page_table, int32_t n_seq, int32_t max_pages, const int32_t *dev_seq, const int32_t *dev_pos,
+    void *dev_q_out, int64_t q_out_stride, int32_t *dev_status, void *stream);
+
+/* Attention of one token of each of n_seq <= 65535 sequences, whose own key
+ * and value are in the cache already: out[t] = softmax(scale q[t] K^T) V over
+ * the keys that position p = positions[t] sees: j <= p, and, with window > 0,
+ * j > p - window or j < n_sink.  scale 0: 1 / sqrt(head_dim).  A negative
+ * position is a padding row and gives zeros.  head_dim 32, 64, 128 or 256; any
+ * number of query heads per kv head; 16-bit rows need a cache of their own
+ * type, f32 rows take any.  out: [n_seq][n_head * head_dim]. */
+SFK_API sfk_status sfk_attn_decode_window(int32_t io_type, const void *dev_q, int64_t q_stride, int32_t kv_type,
+                                          const void *dev_k_pages, const void *dev_v_pages, int32_t n_pages,
+                                          const int32_t *dev_page_table, int32_t max_pages, const int32_t *dev_positions,
+                                          int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                                          float scale, int32_t window, int32_t n_sink, void *dev_out,
+                                          int32_t *dev_status, void *stream);
+
+/* The same attention for the newest tokens of each of n_seq sequences: rows
+ * q_start[s] .. q_start[s+1]-1 of q (q_start [n_seq + 1], ascending, device)
+ * are the last n_q of the kv_len[s] tokens that sequence s has in the cache
+ * (kv_len device), and token i of them sits at position kv_len[s] - n_q + i.
+ * A token whose position is negative sees nothing and gives zeros; rows of q
+ * outside every sequence are neither read nor written.
+ * out: [n_tok][n_head * head_dim]. */
+SFK_API sfk_status sfk_attn_prefill_window(int32_t io_type, const void *dev_q, int64_t q_stride, int32_t n_tok,
+                                           int32_t kv_type, const void *dev_k_pages, const void *dev_v_pages,
+                                           int32_t n_pages, const int32_t *dev_page_table, int32_t max_pages,
+                                           const int32_t *dev_q_start, const int32_t *dev_kv_len, int32_t n_seq,
+                                           int32_t n_head, int32_t n_head_kv, int32_t head_dim, float scale,
+                                           int32_t window, int32_t n_sink, void *dev_out, int32_t *dev_status,
+                                           void *stream);
+
+/* Wait for `stream`, read the paged-cache operators' status word and clear
+ * it: SFK_OK, or SFK_ERR_RUNTIME with what it recorded in sfk_last_error. */
+SFK_API sfk_status sfk_device_status(int32_t *dev_status, void *stream);
 
 #ifdef __cplusplus
 }

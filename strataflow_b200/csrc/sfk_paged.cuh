@@ -1,0 +1,179 @@
+// sfk_paged.cuh -- parameter blocks, launch entry points and shared device
+// code of the operator-level paged-cache kernels: rotated append
+// (sfk_paged_append.cu), windowed attention of single tokens
+// (sfk_paged_decode.cu) and of prompts (sfk_paged_prefill.cu).
+//
+// The cache is the engine's: pools of 16-token pages [page][Hkv][16][hd] for
+// K and V and a table of page ids per sequence.  Key j is seen from position
+// p when j <= p and (window == 0, or j > p - window, or j < n_sink).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "sfk_device.cuh"
+
+namespace sfk {
+
+constexpr int PG = 16;  // tokens per page
+
+// element types of the rows (SFK_TYPE_*) and of the cache (SFK_KV_*), as one enum
+enum Elem : int { EL_F32 = 0, EL_F16 = 1, EL_BF16 = 2 };
+inline int elem_size(int e) { return e == EL_F32 ? 4 : 2; }
+
+constexpr int APPEND_MAX_PAIRS = 128;  // rotated pairs per head (head_dim <= 256)
+
+struct AppendParams {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
+  int n_tok, n_head, n_head_kv, hd;
+  const float *q_norm, *k_norm;  // [hd] or null
+  float eps;
+  int neox, n_rot;
+  const float* freqs;      // [n_rot / 2]
+  const int* rope_pos;     // [n_axes][n_tok] or null: the cache positions
+  int n_axes;
+  void *k_pages, *v_pages;
+  const int* page_table;  // [n_seq][max_pages]
+  int n_seq, max_pages, n_pages;
+  const int* seq;  // [n_tok] or null: token t is sequence t's
+  const int* pos;  // [n_tok]
+  int* status;     // or null
+  int vec;         // 16-byte accesses: bit 0 q, 1 k, 2 v, 3 q_out
+  int lpr;         // lanes per head row (a power of two, 8 elements each)
+  int tpc;         // tokens per CTA
+  uint8_t axis[APPEND_MAX_PAIRS];
+};
+cudaError_t launch_append(AppendParams& p, int io, int kv, int sm_count, cudaStream_t st);
+
+struct WindowAttnParams {
+  const void* q;
+  int64_t q_stride;  // elements between tokens
+  int io;            // Elem of q and out
+  int q_vec;         // q rows are 16-byte aligned
+  const void *k_pages, *v_pages;
+  int n_pages, max_pages, n_head, n_head_kv;
+  const int* page_table;
+  float scale_log2;  // softmax scale * log2(e)
+  int window, n_sink;
+  void* out;         // [tokens][n_head * hd]
+  int* status;       // or null
+  // decode
+  const int* pos;    // [n_seq]
+  int n_seq;
+  int cluster;       // CTAs that share one (sequence, kv head, row tile)
+  // prefill
+  const int* q_start;  // [n_seq + 1]
+  const int* kv_len;   // [n_seq]
+  int n_tok;
+};
+cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
+cudaError_t launch_window_prefill(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
+
+#ifdef __CUDACC__
+// ---- element access -----------------------------------------------------------
+template <class T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+// one rounding to nearest even
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <class T>
+struct Raw8 {  // eight elements as loaded
+  uint4 w[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ void load8(Raw8<T>& r, const T* p, bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+    T* e = reinterpret_cast<T*>(r.w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = p[i];
+  }
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&x)[8]) {
+  const T* e = reinterpret_cast<const T*>(r.w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8], bool vec) {
+  Raw8<T> r;
+  T* e = reinterpret_cast<T*>(r.w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = e[i];
+  }
+}
+// element i of a row of `io` elements, and its store (the type is the same for the whole launch)
+__device__ __forceinline__ float load_elem(const void* p, int64_t i, int io) {
+  if (io == EL_F32) return static_cast<const float*>(p)[i];
+  if (io == EL_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float x, int io) {
+  if (io == EL_F32) static_cast<float*>(p)[i] = x;
+  else if (io == EL_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+}
+
+// 2^x, at most 2 ulp off; 0 for -inf
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void report(int* status, int code) {
+  if (status) atomicExch(status, code);
+}
+
+// The pages a query position (or a run of them) can see: pages 0 .. n_sink_pages-1
+// and pages first .. last, as one list of n entries.
+struct SeenPages {
+  int sink;   // leading pages that only the sinks need (0 when the window reaches them)
+  int first;  // first page of the window
+  int n;      // entries
+  __device__ __forceinline__ int page(int i) const { return i < sink ? i : first + i - sink; }
+};
+// positions lo_pos .. hi_pos (0 <= lo_pos <= hi_pos)
+__device__ __forceinline__ SeenPages seen_pages(int lo_pos, int hi_pos, int window, int n_sink) {
+  SeenPages s;
+  const int lo = window > 0 && lo_pos >= window ? lo_pos - window + 1 : 0;
+  const int last = hi_pos / PG;
+  s.first = lo / PG;
+  const int sp = min((int64_t)last + 1, ((int64_t)n_sink + PG - 1) / PG);
+  s.sink = min(sp, s.first);
+  if (s.sink == s.first) s.sink = s.first = 0;  // one run from page 0
+  s.n = s.sink + last - s.first + 1;
+  return s;
+}
+__device__ __forceinline__ bool key_seen(int j, int p, int window, int n_sink) {
+  return j <= p && (window == 0 || j > p - window || j < n_sink);
+}
+#endif
+
+}  // namespace sfk

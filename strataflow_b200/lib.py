@@ -16,7 +16,8 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "sfk.h")
 SFK_OK = 0
 SFK_ERR_INVALID_ARGUMENT, SFK_ERR_UNSUPPORTED, SFK_ERR_OUT_OF_MEMORY, SFK_ERR_RUNTIME = 1, 3, 4, 7
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K = 0, 1, 8, 12, 14, 15
-KV_F32, KV_F16 = 0, 1
+TYPE_BF16 = 30  # activation rows of the paged-cache operators
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2
 (T_TOK_EMBD, T_OUTPUT_NORM, T_OUTPUT, T_ATTN_NORM, T_ATTN_Q, T_ATTN_K, T_ATTN_V, T_ATTN_OUT,
  T_FFN_NORM, T_FFN_GATE_INP, T_FFN_GATE_EXPS, T_FFN_UP_EXPS, T_FFN_DOWN_EXPS) = range(13)
 LAYERED = set(range(T_ATTN_NORM, 13))
@@ -92,6 +93,13 @@ _SIGS = {
     "sfk_moe_ffn": (I32, [C.c_int, C.c_int, P, P, P, I32, I64, I64, P, P, P, P, I32, I32, P, P]),
     "sfk_moe_ffn_noalloc": (I32, [C.c_int, C.c_int, P, P, P, I32, I64, I64, P, P, P, P, I32, I32, P, P]),
     "sfk_attn_decode_paged": (I32, [P, P, P, I32, I32, P, I32, P, I32, I32, I32, I32, P, P]),
+    "sfk_qk_norm_rope_append": (I32, [I32, P, I64, P, I64, P, I64, I32, I32, I32, I32, P, P, F, I32, I32, P, P, I32,
+                                      P, I32, P, P, I32, P, I32, I32, P, P, P, I64, P, P]),
+    "sfk_attn_decode_window": (I32, [I32, P, I64, I32, P, P, I32, P, I32, P, I32, I32, I32, I32, F, I32, I32, P, P,
+                                     P]),
+    "sfk_attn_prefill_window": (I32, [I32, P, I64, I32, I32, P, P, I32, P, I32, P, P, I32, I32, I32, I32, F, I32, I32,
+                                      P, P, P]),
+    "sfk_device_status": (I32, [P, P]),
     "sfk_ep_handle": (I32, [P, P, SZ]),
     "sfk_ep_connect": (I32, [P, P, I32]),
     "sfk_strata_open": (I32, [C.c_char_p, C.POINTER(P)]),

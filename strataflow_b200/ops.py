@@ -126,3 +126,201 @@ def sample_logits(logits: torch.Tensor, temperature: float, top_k: int = 0, top_
     L.check(L.load().sfk_sample_logits(_ptr(logits), int(logits.numel()), C.byref(sp), int(step), C.byref(tok),
                                        _stream(logits)))
     return tok.value
+
+
+# ---- paged-cache operators (sfk_qk_norm_rope_append, sfk_attn_*_window) ---------
+# They run on the current stream of the tensors' device and return without
+# waiting; nothing is allocated but the output, so they can be captured into a
+# CUDA graph.  Refusals raise SfkError (invalid argument).  `status`, an int32
+# CUDA tensor of one zero, collects what only the device can see (a page id or a
+# position outside its range); check_status reads it.
+_ROW_TYPES = {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
+_KV_TYPES = {torch.float32: L.KV_F32, torch.float16: L.KV_F16, torch.bfloat16: L.KV_BF16}
+
+
+def _refuse(msg: str):
+    raise L.SfkError(L.SFK_ERR_INVALID_ARGUMENT, msg)
+
+
+def _rows(t: torch.Tensor, what: str, heads: int, hd: int, dtype, device) -> tuple[int, int]:
+    """Pointer and token stride of [tokens][heads][hd] rows whose heads are contiguous."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.dtype != dtype or t.device != device:
+        _refuse(f"{what}: {dtype} [tokens][{heads}][{hd}] on {device} is wanted, got {t.dtype} {tuple(t.shape)} on "
+                f"{t.device}")
+    s = t.stride()
+    if (s[2] != 1 and hd > 1) or (s[1] != hd and heads > 1):
+        _refuse(f"{what}: a token's heads have to be contiguous, got strides {s}")
+    return t.data_ptr(), (s[0] if t.shape[0] > 1 else max(s[0], heads * hd))
+
+
+def _int32(t: torch.Tensor, what: str, shape, device) -> int:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        _refuse(f"{what}: contiguous int32 {list(shape)} on {device} is wanted, got {t.dtype} {list(t.shape)} on "
+                f"{t.device}")
+    return t.data_ptr()
+
+
+def _f32(t: torch.Tensor | None, what: str, n: int, device) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        _refuse(f"{what}: contiguous float32 [{n}] on {device} is wanted, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, device) -> tuple[int, int, int]:
+    """(kv type, kv heads, head_dim) of a checked cache."""
+    if (k_pages.dim() != 4 or k_pages.shape[2] != 16 or k_pages.shape != v_pages.shape or
+            k_pages.dtype != v_pages.dtype or k_pages.dtype not in _KV_TYPES):
+        _refuse(f"page pools: two [n_pages][n_head_kv][16][head_dim] of one type (f32, f16, bf16) are wanted, got "
+                f"{k_pages.dtype} {tuple(k_pages.shape)} and {v_pages.dtype} {tuple(v_pages.shape)}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()) or k_pages.device != device or v_pages.device != device:
+        _refuse(f"page pools: contiguous and on {device}")
+    if page_table.dim() != 2:
+        _refuse("page_table: [n_seq][max_pages] is wanted")
+    return _KV_TYPES[k_pages.dtype], k_pages.shape[1], k_pages.shape[3]
+
+
+def _cuda_device(t: torch.Tensor, what: str):
+    if not t.is_cuda:
+        _refuse(f"{what}: a CUDA tensor is wanted, got one on {t.device}")
+    return t.device
+
+
+def _call(device, fn, *args) -> None:
+    """Run an entry on `device`'s current stream (the library launches on the current device)."""
+    if device.index == torch.cuda.current_device():
+        L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _status(status: torch.Tensor | None, device) -> int | None:
+    return None if status is None else _int32(status, "status", (1,), device)
+
+
+def check_status(status: torch.Tensor) -> None:
+    """Wait for the current stream; raise SfkError if the status word of earlier
+    paged-cache calls records an error, and clear it."""
+    device = _cuda_device(status, "status")
+    _call(device, L.load().sfk_device_status, _status(status, device))
+
+
+def rope_freqs(n_rot: int, base: float = 10000.0, scale: float = 1.0, device="cuda") -> torch.Tensor:
+    """Rotation frequencies base^(-2i / n_rot) * scale, f32 [n_rot / 2]."""
+    i = torch.arange(n_rot // 2, dtype=torch.float64)
+    return (base ** (-2 * i / n_rot) * scale).to(torch.float32).to(device)
+
+
+def rope_axes(sections, interleaved: bool = False) -> bytes:
+    """The axis of each pair: `sections[a]` pairs on axis a, in runs, or dealt
+    out in turn (each axis as long as it has pairs left) when interleaved."""
+    if not interleaved:
+        return bytes(a for a, n in enumerate(sections) for _ in range(n))
+    left, out = list(sections), []
+    while any(left):
+        for a in range(len(left)):
+            if left[a]:
+                left[a] -= 1
+                out.append(a)
+    return bytes(out)
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
+                        v_pages: torch.Tensor, page_table: torch.Tensor, pos: torch.Tensor, *,
+                        seq: torch.Tensor | None = None, freqs: torch.Tensor | None = None, neox: bool = False,
+                        q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                        rope_pos: torch.Tensor | None = None, axes: bytes | None = None,
+                        out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """sfk_qk_norm_rope_append: norm (q_norm / k_norm [hd]) and rotate
+    (freqs [n_rot / 2], None: no rotation) the heads of q [tokens][Hq][hd] and
+    k [tokens][Hkv][hd], append k and v to the cache at position pos[t] of
+    sequence seq[t] (None: t), and return the rotated q (`out`, which may be
+    q).  rope_pos [n_axes][tokens] with axes (rope_axes) replaces the cache
+    positions in the rotation.  Rows with pos < 0 are padding."""
+    dev = _cuda_device(q, "q")
+    kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
+    n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    if q.dtype not in _ROW_TYPES:
+        _refuse(f"q: f32, f16 or bf16 is wanted, got {q.dtype}")
+    qp, qs = _rows(q, "q", heads, hd, q.dtype, dev)
+    kp, ks = _rows(k, "k", kvh, hd, q.dtype, dev)
+    vp, vs = _rows(v, "v", kvh, hd, q.dtype, dev)
+    if k.shape[0] != n or v.shape[0] != n:
+        _refuse(f"q, k and v: {n}, {k.shape[0]} and {v.shape[0]} tokens")
+    if out is None:
+        out = torch.empty((n, heads, hd), dtype=q.dtype, device=dev)
+    op, os_ = _rows(out, "out", heads, hd, q.dtype, dev)
+    if out.shape[0] != n:
+        _refuse(f"out: {n} tokens are wanted, got {out.shape[0]}")
+    n_rot = 0 if freqs is None else 2 * freqs.numel()
+    n_axes = 0
+    if rope_pos is not None:
+        n_axes = rope_pos.shape[0] if rope_pos.dim() == 2 else 0
+        _int32(rope_pos, "rope_pos", (n_axes, n), dev)
+    if axes is not None and len(axes) != n_rot // 2:
+        _refuse(f"axes: {n_rot // 2} pairs are rotated, got {len(axes)}")
+    n_seq = page_table.shape[0]
+    _call(dev, L.load().sfk_qk_norm_rope_append, _ROW_TYPES[q.dtype], qp, qs, kp, ks, vp, vs, n, heads, kvh, hd,
+          _f32(q_norm, "q_norm", hd, dev), _f32(k_norm, "k_norm", hd, dev), eps, int(neox), n_rot,
+          _f32(freqs, "freqs", n_rot // 2, dev), None if rope_pos is None else rope_pos.data_ptr(), n_axes, axes, kvt,
+          k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
+          _int32(page_table, "page_table", (n_seq, page_table.shape[1]), dev), n_seq, page_table.shape[1],
+          None if seq is None else _int32(seq, "seq", (n,), dev), _int32(pos, "pos", (n,), dev), op, os_,
+          _status(status, dev))
+    return out
+
+
+def _attn_rows(q: torch.Tensor, k_pages: torch.Tensor, kvh: int, hd: int, window: int, n_sink: int,
+               out: torch.Tensor | None, dev):
+    if not (0 <= window < 1 << 31 and 0 <= n_sink < 1 << 31):
+        _refuse(f"window {window}, n_sink {n_sink}")
+    heads = q.shape[1] if q.dim() == 3 else 0
+    if q.dtype not in _ROW_TYPES:
+        _refuse(f"q: f32, f16 or bf16 is wanted, got {q.dtype}")
+    if q.dtype != torch.float32 and q.dtype != k_pages.dtype:
+        _refuse(f"q: {q.dtype} rows need a cache of their own type, got {k_pages.dtype}")
+    qp, qs = _rows(q, "q", heads, hd, q.dtype, dev)
+    shape = (q.shape[0], heads * hd)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or tuple(out.shape) != shape or out.device != dev or not out.is_contiguous():
+        _refuse(f"out: contiguous {q.dtype} {list(shape)} on {dev} is wanted")
+    return heads, qp, qs, out
+
+
+def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                       positions: torch.Tensor, *, window: int = 0, n_sink: int = 0, scale: float = 0.0,
+                       out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """sfk_attn_decode_window: q [n_seq][Hq][hd], one token of each sequence at
+    positions[t] (negative: padding, zeros) over the keys it sees: j <= p and,
+    with window > 0, j > p - window or j < n_sink.  Returns [n_seq][Hq * hd]."""
+    dev = _cuda_device(q, "q")
+    kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
+    heads, qp, qs, out = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
+    n = q.shape[0]
+    _call(dev, L.load().sfk_attn_decode_window, _ROW_TYPES[q.dtype], qp, qs, kvt, k_pages.data_ptr(),
+          v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
+          page_table.shape[1], _int32(positions, "positions", (n,), dev), n, heads, kvh, hd, scale, window, n_sink,
+          out.data_ptr(), _status(status, dev))
+    return out
+
+
+def attn_prefill_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                        q_start: torch.Tensor, kv_len: torch.Tensor, *, window: int = 0, n_sink: int = 0,
+                        scale: float = 0.0, out: torch.Tensor | None = None,
+                        status: torch.Tensor | None = None) -> torch.Tensor:
+    """sfk_attn_prefill_window: rows q_start[s] .. q_start[s+1]-1 of q
+    [tokens][Hq][hd] are the newest of the kv_len[s] tokens of sequence s in
+    the cache; each attends over the keys it sees (attn_decode_window).
+    Returns [tokens][Hq * hd]; rows of no sequence are not written."""
+    dev = _cuda_device(q, "q")
+    kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
+    heads, qp, qs, out = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
+    n = page_table.shape[0]
+    _call(dev, L.load().sfk_attn_prefill_window, _ROW_TYPES[q.dtype], qp, qs, q.shape[0], kvt, k_pages.data_ptr(),
+          v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
+          page_table.shape[1], _int32(q_start, "q_start", (n + 1,), dev), _int32(kv_len, "kv_len", (n,), dev), n, heads,
+          kvh, hd, scale, window, n_sink, out.data_ptr(), _status(status, dev))
+    return out
