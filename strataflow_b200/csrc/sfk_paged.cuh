@@ -53,7 +53,7 @@ struct WindowAttnParams {
   const void* q;
   int64_t q_stride;  // elements between tokens
   int io;            // Elem of q and out
-  int q_vec;         // q rows are 16-byte aligned
+  int q_vec, out_vec;  // rows are 16-byte aligned
   const void *k_pages, *v_pages;
   int n_pages, max_pages, n_head, n_head_kv;
   const int* page_table;
@@ -72,6 +72,9 @@ struct WindowAttnParams {
 };
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
 cudaError_t launch_window_prefill(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
+// the tensor-core form: whether it takes these types and sizes, and its launch
+bool prefill_tc_takes(const WindowAttnParams& p, int kv, int hd);
+cudaError_t launch_prefill_tc(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
 
 #ifdef __CUDACC__
 // ---- element access -----------------------------------------------------------
@@ -173,6 +176,57 @@ __device__ __forceinline__ SeenPages seen_pages(int lo_pos, int hi_pos, int wind
 }
 __device__ __forceinline__ bool key_seen(int j, int p, int window, int n_sink) {
   return j <= p && (window == 0 || j > p - window || j < n_sink);
+}
+
+// Tile `idx` of the ragged batch: tiles of RT rows, sequence by sequence, the
+// last tile of a sequence first (its rows see the most keys).  All lanes of
+// the warp call it and get the same answer; seq = -1 past the last tile.
+struct Tile {
+  int seq, q0, n_q, row0;  // first token of the sequence, its tokens, first row
+  int past;                // position of its first token
+};
+template <int RT>
+__device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx) {
+  const int lane = threadIdx.x & 31;
+  const int64_t group = p.n_head / p.n_head_kv;
+  Tile t;
+  t.seq = -1;
+  for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
+    const int s = s0 + lane;
+    int a = 0, n = 0, len = 0;
+    int64_t tiles = 0;
+    if (s < p.n_seq) {
+      a = p.q_start[s];
+      const int b = p.q_start[s + 1];
+      len = p.kv_len[s];
+      if (a < 0 || b < a || b > p.n_tok || len < 0 || (len + PG - 1) / PG > p.max_pages) {
+        report(p.status, ERR_BAD_POS);  // nothing of this sequence is read or written
+      } else {
+        n = b - a;
+        tiles = (n * group + RT - 1) / RT;
+      }
+    }
+    int64_t incl = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, idx < incl);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t before = __shfl_sync(0xffffffffu, incl - tiles, src);
+      const int64_t cnt = __shfl_sync(0xffffffffu, tiles, src);
+      t.seq = s0 + src;
+      t.q0 = __shfl_sync(0xffffffffu, a, src);
+      t.n_q = __shfl_sync(0xffffffffu, n, src);
+      t.past = __shfl_sync(0xffffffffu, len, src) - t.n_q;
+      t.row0 = (int)((cnt - 1 - (idx - before)) * RT);
+      return t;
+    }
+    idx -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return t;
 }
 #endif
 

@@ -73,6 +73,7 @@ sfk_status attn_args(const char* who, WindowAttnParams& a, int* kv, int32_t io_t
   a.q_stride = q_stride;
   a.io = io;
   a.q_vec = vec_rows(q, q_stride, io);
+  a.out_vec = aligned16(out);
   a.k_pages = kp;
   a.v_pages = vp;
   a.n_pages = n_pages;

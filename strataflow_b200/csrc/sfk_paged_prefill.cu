@@ -13,57 +13,6 @@
 namespace sfk {
 namespace {
 
-// Tile `idx` of the ragged batch: tiles of RT rows, sequence by sequence, the
-// last tile of a sequence first (its rows see the most keys).  All lanes of
-// the warp call it and get the same answer; seq = -1 past the last tile.
-struct Tile {
-  int seq, q0, n_q, row0;  // first token of the sequence, its tokens, first row
-  int past;                // position of its first token
-};
-template <int RT>
-__device__ Tile find_tile(const WindowAttnParams& p, int64_t idx) {
-  const int lane = threadIdx.x & 31;
-  const int64_t group = p.n_head / p.n_head_kv;
-  Tile t;
-  t.seq = -1;
-  for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
-    const int s = s0 + lane;
-    int a = 0, n = 0, len = 0;
-    int64_t tiles = 0;
-    if (s < p.n_seq) {
-      a = p.q_start[s];
-      const int b = p.q_start[s + 1];
-      len = p.kv_len[s];
-      if (a < 0 || b < a || b > p.n_tok || len < 0 || (len + PG - 1) / PG > p.max_pages) {
-        report(p.status, ERR_BAD_POS);  // nothing of this sequence is read or written
-      } else {
-        n = b - a;
-        tiles = (n * group + RT - 1) / RT;
-      }
-    }
-    int64_t incl = tiles;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, idx < incl);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int64_t before = __shfl_sync(0xffffffffu, incl - tiles, src);
-      const int64_t cnt = __shfl_sync(0xffffffffu, tiles, src);
-      t.seq = s0 + src;
-      t.q0 = __shfl_sync(0xffffffffu, a, src);
-      t.n_q = __shfl_sync(0xffffffffu, n, src);
-      t.past = __shfl_sync(0xffffffffu, len, src) - t.n_q;
-      t.row0 = (int)((cnt - 1 - (idx - before)) * RT);
-      return t;
-    }
-    idx -= __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return t;
-}
-
 // ---- CUDA cores: any cache type ------------------------------------------------------
 // 64 rows x 64 keys per step, 256 threads as 16 x 16: thread (ty, tx) owns rows
 // ty + 16 i, keys tx + 16 j of the scores and dims 4 tx .. 4 tx + 3 of each 64
@@ -257,7 +206,7 @@ cudaError_t launch_kv(WindowAttnParams& p, int hd, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_window_prefill(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {
-  (void)sm_count;
+  if (prefill_tc_takes(p, kv, hd)) return launch_prefill_tc(p, kv, hd, sm_count, st);
   if (kv == EL_F32) return launch_kv<float>(p, hd, st);
   if (kv == EL_F16) return launch_kv<__half>(p, hd, st);
   return launch_kv<__nv_bfloat16>(p, hd, st);
