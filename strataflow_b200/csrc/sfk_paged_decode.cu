@@ -13,6 +13,8 @@
 // several graphs have nothing in common.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "sfk_paged.cuh"
 
 namespace sfk {
@@ -20,13 +22,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int DW = 4;         // warps per CTA
-constexpr int DT = DW * 32;
 
 // ---- join -----------------------------------------------------------------------
 // Every warp's partial (m, l, o) of R rows to the output.  m is in units of
 // log2; a partial without keys has m = -inf, l = 0, o = 0.
-template <int R, int HD>
+template <int R, int HD, int DW>
 struct JoinSmem {
   float o[DW][R][HD];
   float m[DW][R], l[DW][R];
@@ -34,8 +34,9 @@ struct JoinSmem {
   float cm[R], cl[R];
 };
 
-template <int R, int HD>
-__device__ void join_and_store(JoinSmem<R, HD>& sm, const WindowAttnParams& p, int seq, int head0, int n_rows, bool any) {
+template <int R, int HD, int DW>
+__device__ void join_and_store(JoinSmem<R, HD, DW>& sm, const WindowAttnParams& p, int seq, int head0, int n_rows, bool any) {
+  constexpr int DT = DW * 32;
   cg::cluster_group cl = cg::this_cluster();
   const int C = p.cluster, rank = C > 1 ? (int)cl.block_rank() : 0;
   const int tid = threadIdx.x;
@@ -130,16 +131,16 @@ __device__ __forceinline__ int page_id(const WindowAttnParams& p, const Work& w,
 // rows in shared memory.  Values: the lane owns HD / 32 output dims.
 template <class KV, int HD>
 struct CcSmem {
-  static constexpr int R = 8;
+  static constexpr int R = 8, DW = 4;
   float q[R][HD];
   float p[DW][R][PG];
-  JoinSmem<R, HD> join;
+  JoinSmem<R, HD, DW> join;
 };
 
 template <class KV, int HD>
-__global__ void __launch_bounds__(DT) decode_cc_kernel(const __grid_constant__ WindowAttnParams p) {
+__global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(const __grid_constant__ WindowAttnParams p) {
   using Smem = CcSmem<KV, HD>;
-  constexpr int R = Smem::R, E = HD / 32;
+  constexpr int R = Smem::R, E = HD / 32, DW = Smem::DW, DT = DW * 32;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
@@ -242,8 +243,248 @@ __global__ void __launch_bounds__(DT) decode_cc_kernel(const __grid_constant__ W
   join_and_store(sm.join, p, w.seq, w.head0, w.n_rows, w.pos >= 0);
 }
 
+// ---- tensor cores (mma.sync): 16-bit caches ------------------------------------------
+// A warp takes a page (16 keys) at a time, its K and V rows straight from global
+// memory into the B operands of m16n8k16 products, no shared memory between:
+//   S (8 heads x 16 keys): the operand's inner index is a permutation of the head
+//   dims that q follows too, so lane (g, t) holds dims 8 t .. 8 t + 7 of each 32 of
+//   keys g and g + 8, one 16-byte load per 32 dims and key.
+//   O (8 heads x hd): lane (g, t) loads V of keys 2t, 2t+1, 2t+8, 2t+9, dims
+//   VE g .. of each 8 VE; a byte permute of two keys' words gives the operand.
+// The product has 16 rows and a CTA takes 8 heads: the other 8 rows carry what f32
+// has below 16 bits.  Rows 0-7 hold the first term of q (32-bit rows: q scaled by a
+// power of two per head, as two f16 terms) and of P, rows 8-15 the second; the two
+// halves of S and of O are added.  P reaches 2^BIAS, so that its second term keeps
+// clear of f16's smallest step; the running maximum moves when a row outgrows it by
+// 2^RAISE.
+constexpr int MMA_R = 8;
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (x, y) rounded to 16 bits in one word, and what the rounding left, in another
+template <bool BF16>
+__device__ __forceinline__ void two_terms(float x, float y, uint32_t& hi, uint32_t& lo) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  }
+}
+template <int N>
+__device__ __forceinline__ void ldg_words(uint32_t (&r)[N], const void* p) {
+  if constexpr (N == 4)
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "l"(p));
+  else
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+}
+
+template <int HD, int DW>
+struct MmaSmem {
+  uint4 q[HD / 16][32];  // A operands of q, by lane
+  float up[MMA_R];       // scale of each head's scores
+  JoinSmem<MMA_R, HD, DW> join;
+};
+
+template <class KV, int HD, bool SPLIT, int DW>
+__global__ void __launch_bounds__(DW * 32, HD > 128 ? 8 / DW : 12 / DW)
+    decode_mma_kernel(const __grid_constant__ WindowAttnParams p) {
+  constexpr bool BF16 = std::is_same<KV, __nv_bfloat16>::value;
+  constexpr int DT = DW * 32;
+  constexpr int KC = HD / 32;                    // 32-dim chunks of K
+  constexpr int VE = HD / 8 < 8 ? HD / 8 : 8;    // dims per V load
+  constexpr int VC = HD / (8 * VE);              // V loads per key
+  constexpr float RAISE = 4.f, BIAS = 11.f;
+  using Smem = MmaSmem<HD, DW>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  const Work w = find_work<MMA_R>(p);
+
+  // page ids of this warp's entries i0 + warp + DW k, 32 at a time
+  int ids = 0, ids_at = 0;
+  auto fetch_ids = [&](int k0) {
+    const int i = w.i0 + warp + DW * (k0 + lane);
+    ids = i < w.i1 ? page_id(p, w, i) : -1;
+    ids_at = k0;
+  };
+  const int mine = (w.i1 - w.i0 - warp + DW - 1) / DW;  // pages of this warp (<= 0: none)
+  if (mine > 0) fetch_ids(0);
+  const int64_t head_bytes = (int64_t)w.hk * PG * HD * 2, page_bytes = (int64_t)p.n_head_kv * PG * HD * 2;
+  // an id outside the pool reads page 0, and its keys count as masked
+  auto offset = [&](int k) { return (int64_t)max(__shfl_sync(0xffffffffu, ids, k - ids_at), 0) * page_bytes + head_bytes; };
+  uint32_t kr[KC][2][4], vr[4][VC][VE / 2];
+  auto load_k = [&](int64_t off) {
+    const uint8_t* b = static_cast<const uint8_t*>(p.k_pages) + off + g * (HD * 2) + t * 16;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      ldg_words(kr[c][0], b + c * 64);
+      ldg_words(kr[c][1], b + 8 * HD * 2 + c * 64);
+    }
+  };
+  auto load_v = [&](int64_t off) {
+    const uint8_t* b = static_cast<const uint8_t*>(p.v_pages) + off + 2 * t * (HD * 2) + g * (VE * 2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < VC; ++c) ldg_words(vr[j][c], b + ((j & 1) + (j & 2) * 4) * (HD * 2) + c * (16 * VE));
+  };
+  // The next page's K is requested as soon as this page's is used up, its V
+  // likewise, so one of the two is always on its way.  At hd 256 the registers
+  // do not hold that: both are requested together when their page begins.
+  constexpr bool AHEAD = HD <= 128;
+  if (AHEAD && mine > 0) {
+    const int64_t off = offset(0);
+    load_k(off);
+    load_v(off);
+  }
+
+  // q as A operands: k-step s, lane (g, t): dims 32 (s / 2) + 8 t + 4 (s % 2) + 0..3
+  if (SPLIT && warp < MMA_R) {
+    for (int r = warp; r < MMA_R; r += DW) {
+      float mx = 0.f;
+      if (r < w.n_rows)
+        for (int d = lane; d < HD; d += 32)
+          mx = fmaxf(mx, fabsf(load_elem(p.q, w.seq * p.q_stride + (int64_t)(w.head0 + r) * HD + d, p.io)));
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const int e = (int)(__float_as_uint(mx) >> 23) - 127;  // largest |q| to [1, 2): exact
+      if (lane == 0) sm.up[r] = mx > 0.f && e < 128 ? exp2f((float)max(e, -126)) : 1.f;
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < HD / 16 * 32; i += DT) {
+    const int s = i / 32, gg = i % 32 / 4, tt = i % 4;
+    float x[4] = {};
+    if (gg < w.n_rows) {
+      const int64_t at = w.seq * p.q_stride + (int64_t)(w.head0 + gg) * HD + s / 2 * 32 + tt * 8 + s % 2 * 4;
+      const float down = SPLIT ? 1.f / sm.up[gg] : 1.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = load_elem(p.q, at + e, p.io) * down;
+    }
+    uint4 a;
+    two_terms<BF16>(x[0], x[1], a.x, a.y);  // 16-bit rows: the second term is 0
+    two_terms<BF16>(x[2], x[3], a.z, a.w);
+    sm.q[s][i % 32] = a;
+  }
+  __syncthreads();
+  const float scale = p.scale_log2 * (SPLIT ? sm.up[g] : 1.f);
+
+  float o[VC * VE][4];
+#pragma unroll
+  for (int i = 0; i < VC * VE; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m = -INFINITY, l = 0.f;  // of head g; l of this lane's keys
+  for (int k = 0; k < mine; ++k) {
+    const int entry = w.i0 + warp + DW * k, j0 = w.sp.page(entry) * PG;
+    if (!AHEAD && k - ids_at == 32) fetch_ids(k);
+    const bool bad = __shfl_sync(0xffffffffu, ids, k - ids_at) < 0;
+    if (!AHEAD) {
+      const int64_t off = offset(k);
+      load_k(off);
+      load_v(off);
+    }
+    float s0[4] = {}, s1[4] = {};
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 q = sm.q[2 * c + h][lane];
+        const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+        mma16816<BF16>(s0, a, kr[c][0][2 * h], kr[c][0][2 * h + 1]);
+        mma16816<BF16>(s1, a, kr[c][1][2 * h], kr[c][1][2 * h + 1]);
+      }
+    int64_t next = 0;
+    if (AHEAD && k + 1 < mine) {
+      if (k + 1 - ids_at == 32) fetch_ids(k + 1);
+      next = offset(k + 1);
+      load_k(next);
+    }
+    // keys 2t, 2t+1, 2t+8, 2t+9 of head g
+    float x[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+    const bool edge = bad || j0 + PG - 1 > w.pos || (p.window > 0 && j0 <= w.pos - p.window);
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool see = !bad && key_seen(j0 + 2 * t + (j & 1) + (j & 2) * 4, w.pos, p.window, p.n_sink);
+        if (!see) {
+          x[j] = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < VC; ++c)  // whatever a masked place holds is not used
+#pragma unroll
+            for (int e = 0; e < VE / 2; ++e) vr[j][c][e] = 0;
+        }
+      }
+    }
+    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * scale;
+    if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
+      const float mn = fmaxf(mx, m);
+      const float f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < VC * VE; ++i) {
+        o[i][0] *= f;
+        o[i][1] *= f;
+        o[i][2] *= f;
+        o[i][3] *= f;
+      }
+    }
+    const float neg = BIAS - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = exp2_approx(fmaf(x[j], scale, neg));
+    l += (x[0] + x[1]) + (x[2] + x[3]);
+    uint32_t a[4];
+    two_terms<BF16>(x[0], x[1], a[0], a[1]);
+    two_terms<BF16>(x[2], x[3], a[2], a[3]);
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+        mma16816<BF16>(o[c * VE + e], a, __byte_perm(vr[0][c][e / 2], vr[1][c][e / 2], sel),
+                       __byte_perm(vr[2][c][e / 2], vr[3][c][e / 2], sel));
+      }
+    if (AHEAD && k + 1 < mine) load_v(next);
+  }
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  if (t == 0) {
+    sm.join.m[warp][g] = m;
+    sm.join.l[warp][g] = l;
+  }
+#pragma unroll
+  for (int c = 0; c < VC; ++c)
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      float* dst = &sm.join.o[warp][g][c * 8 * VE + 2 * t * VE + e];
+      dst[0] = o[c * VE + e][0] + o[c * VE + e][2];
+      dst[VE] = o[c * VE + e][1] + o[c * VE + e][3];
+    }
+  join_and_store(sm.join, p, w.seq, w.head0, w.n_rows, w.pos >= 0);
+}
+
 template <class K>
-cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, size_t smem, cudaStream_t st) {
+cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   if (p.cluster > 8) {
@@ -252,7 +493,7 @@ cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, size
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.n_head_kv * tiles * p.cluster), (unsigned)p.n_seq);
-  cfg.blockDim = dim3(DT);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -264,17 +505,18 @@ cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, size
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-// CTAs per (sequence, kv head, row tile): enough for two on every SM, as long
-// as each of a CTA's warps has a page or more.
-int pick_cluster(const WindowAttnParams& p, int tiles, int sm_count) {
-  int64_t pages = p.max_pages;
-  if (p.window > 0)
-    pages = pages < (p.window + PG - 1) / PG + 1 + ((int64_t)p.n_sink + PG - 1) / PG
-                ? pages
-                : (p.window + PG - 1) / PG + 1 + ((int64_t)p.n_sink + PG - 1) / PG;
-  const int64_t pairs = (int64_t)p.n_seq * p.n_head_kv * tiles;
+// pages that the longest possible context of this call sees
+int64_t max_seen_pages(const WindowAttnParams& p) {
+  if (p.window <= 0) return p.max_pages;
+  const int64_t n = (p.window + (int64_t)PG - 1) / PG + 1 + ((int64_t)p.n_sink + PG - 1) / PG;
+  return n < p.max_pages ? n : p.max_pages;
+}
+// CTAs per (sequence, kv head, row tile): enough for `want` in all, as long as
+// each warp has a page or more.
+int pick_cluster(const WindowAttnParams& p, int tiles, int warps, int64_t want) {
+  const int64_t pages = max_seen_pages(p), pairs = (int64_t)p.n_seq * p.n_head_kv * tiles;
   int c = 1;
-  while (c < 16 && pairs * c < 2 * sm_count && pages > (int64_t)c * DW) c *= 2;
+  while (c < 16 && pairs * c < want && pages > (int64_t)c * warps) c *= 2;
   return c;
 }
 
@@ -282,27 +524,45 @@ template <class KV, int HD>
 cudaError_t launch_cc(WindowAttnParams& p, int sm_count, cudaStream_t st) {
   using Smem = CcSmem<KV, HD>;
   const int tiles = (p.n_head / p.n_head_kv + Smem::R - 1) / Smem::R;
-  p.cluster = pick_cluster(p, tiles, sm_count);
-  return launch_clusters(decode_cc_kernel<KV, HD>, p, tiles, sizeof(Smem), st);
+  p.cluster = pick_cluster(p, tiles, Smem::DW, 2 * sm_count);
+  return launch_clusters(decode_cc_kernel<KV, HD>, p, tiles, Smem::DW * 32, sizeof(Smem), st);
 }
 
-template <class KV>
-cudaError_t launch_kv(WindowAttnParams& p, int hd, int sm_count, cudaStream_t st) {
-  switch (hd) {
-    case 32: return launch_cc<KV, 32>(p, sm_count, st);
-    case 64: return launch_cc<KV, 64>(p, sm_count, st);
-    case 128: return launch_cc<KV, 128>(p, sm_count, st);
-    case 256: return launch_cc<KV, 256>(p, sm_count, st);
-  }
-  return cudaErrorInvalidValue;
+template <class KV, int HD, bool SPLIT, int DW>
+cudaError_t launch_mma(WindowAttnParams& p, int tiles, cudaStream_t st) {
+  return launch_clusters(decode_mma_kernel<KV, HD, SPLIT, DW>, p, tiles, DW * 32, sizeof(MmaSmem<HD, DW>), st);
+}
+template <class KV, int HD>
+cudaError_t launch_16(WindowAttnParams& p, int sm_count, cudaStream_t st) {
+  const int tiles = (p.n_head / p.n_head_kv + MMA_R - 1) / MMA_R;
+  const bool split = p.io == EL_F32;
+  // Two or more CTAs of four warps for every SM if the batch gives them, else CTAs of eight warps
+  p.cluster = pick_cluster(p, tiles, 4, 3 * sm_count);
+  const int64_t ctas = (int64_t)p.n_seq * p.n_head_kv * tiles * p.cluster;
+  if (ctas >= 2 * sm_count || max_seen_pages(p) < p.cluster * 8)
+    return split ? launch_mma<KV, HD, true, 4>(p, tiles, st) : launch_mma<KV, HD, false, 4>(p, tiles, st);
+  return split ? launch_mma<KV, HD, true, 8>(p, tiles, st) : launch_mma<KV, HD, false, 8>(p, tiles, st);
+}
+
+template <int HD>
+cudaError_t launch_hd(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
+  if (kv == EL_F32) return launch_cc<float, HD>(p, sm_count, st);
+  if (kv == EL_F16) return launch_16<__half, HD>(p, sm_count, st);
+  // 32-bit rows over a bf16 cache: two bf16 terms hold 16 bits only, so these stay on the CUDA cores
+  if (p.io == EL_F32) return launch_cc<__nv_bfloat16, HD>(p, sm_count, st);
+  return launch_16<__nv_bfloat16, HD>(p, sm_count, st);
 }
 
 }  // namespace
 
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {
-  if (kv == EL_F32) return launch_kv<float>(p, hd, sm_count, st);
-  if (kv == EL_F16) return launch_kv<__half>(p, hd, sm_count, st);
-  return launch_kv<__nv_bfloat16>(p, hd, sm_count, st);
+  switch (hd) {
+    case 32: return launch_hd<32>(p, kv, sm_count, st);
+    case 64: return launch_hd<64>(p, kv, sm_count, st);
+    case 128: return launch_hd<128>(p, kv, sm_count, st);
+    case 256: return launch_hd<256>(p, kv, sm_count, st);
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace sfk
