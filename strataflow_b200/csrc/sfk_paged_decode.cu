@@ -16,12 +16,25 @@
 #include <type_traits>
 
 #include "sfk_paged.cuh"
+#include "sfk_paged_map.cuh"
 
 namespace sfk {
 namespace {
 
 namespace cg = cooperative_groups;
 
+
+// Bounded wait of a whole warp for a slot (about a second); one answer for all lanes.
+__device__ __forceinline__ bool wait_slot(uint64_t* bar, uint32_t parity, int* status) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < (1ll << 31)) {
+    }
+    if (!ok) report(status, ERR_TIMEOUT);
+  }
+  return __all_sync(0xffffffffu, ok);
+}
 
 // ---- join -----------------------------------------------------------------------
 // Every warp's partial (m, l, o) of R rows to the output.  m is in units of
@@ -244,13 +257,17 @@ __global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(cons
 }
 
 // ---- tensor cores (mma.sync): 16-bit caches ------------------------------------------
-// A warp takes a page (16 keys) at a time, its K and V rows straight from global
-// memory into the B operands of m16n8k16 products, no shared memory between:
-//   S (8 heads x 16 keys): the operand's inner index is a permutation of the head
-//   dims that q follows too, so lane (g, t) holds dims 8 t .. 8 t + 7 of each 32 of
-//   keys g and g + 8, one 16-byte load per 32 dims and key.
-//   O (8 heads x hd): lane (g, t) loads V of keys 2t, 2t+1, 2t+8, 2t+9, dims
-//   VE g .. of each 8 VE; a byte permute of two keys' words gives the operand.
+// A warp takes a page (16 keys) at a time.  Each warp has a ring of its own of
+// page slots in shared memory, filled by one tensor-map copy for K and one for V
+// (4 KB each at hd 128, 128-byte swizzle): only lanes of one warp wait for one
+// another, and the bytes under way do not depend on registers.  The operands of
+// the m16n8k16 products come from the slots with 16-byte loads free of bank
+// conflicts, without ldmatrix, because the inner index may be permuted:
+//   S (8 heads x 16 keys): lane (g, t) loads 16-byte chunk 2t + h of each 128
+//   bytes of keys g and g + 8; q follows the same permutation of head dims.
+//   O (8 heads x hd): lane (g, t) loads chunk g of keys 2t, 2t+1, 2t+8, 2t+9; a
+//   byte permute of two keys' words gives the operand, column g of product e
+//   being dim 8 g + e.
 // The product has 16 rows and a CTA takes 8 heads: the other 8 rows carry what f32
 // has below 16 bits.  Rows 0-7 hold the first term of q (32-bit rows: q scaled by a
 // power of two per head, as two f16 terms) and of P, rows 8-15 the second; the two
@@ -287,78 +304,79 @@ __device__ __forceinline__ void two_terms(float x, float y, uint32_t& hi, uint32
     lo = *reinterpret_cast<const uint32_t*>(&l);
   }
 }
-template <int N>
-__device__ __forceinline__ void ldg_words(uint32_t (&r)[N], const void* p) {
-  if constexpr (N == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "l"(p));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
-}
 
 template <int HD, int DW>
+struct MmaCfg {
+  static constexpr int HDP = HD < 64 ? 64 : HD;    // head width in a slot (the copy fills with zeros)
+  static constexpr int PAGE = PG * HDP * 2;        // bytes of a page's K or V
+  static constexpr int FIT = 96 * 1024 / (4 * 2 * PAGE);
+  static constexpr int STAGES = FIT < 3 ? 3 : FIT; // slots per warp: 24 KB of copies under way, or three pages
+  static constexpr int RING = DW * STAGES * 2 * PAGE;
+};
+template <int HD, int DW>
 struct MmaSmem {
-  uint4 q[HD / 16][32];  // A operands of q, by lane
-  float up[MMA_R];       // scale of each head's scores
-  JoinSmem<MMA_R, HD, DW> join;
+  using C = MmaCfg<HD, DW>;
+  union {
+    uint8_t ring[C::RING];  // [warp][stage][K | V][64-dim block][16 keys][128 B]
+    JoinSmem<MMA_R, HD, DW> join;
+  };
+  uint4 q[C::HDP / 16][32];  // A operands of q, by lane
+  float up[MMA_R];           // scale of each head's scores
+  uint64_t full[DW][C::STAGES];
 };
 
 template <class KV, int HD, bool SPLIT, int DW>
-__global__ void __launch_bounds__(DW * 32, HD > 128 ? 8 / DW : 12 / DW)
-    decode_mma_kernel(const __grid_constant__ WindowAttnParams p) {
+__global__ void __launch_bounds__(DW * 32, HD <= 128 && DW == 4 ? 2 : 1)
+    decode_mma_kernel(const __grid_constant__ WindowAttnParams p, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap) {
   constexpr bool BF16 = std::is_same<KV, __nv_bfloat16>::value;
-  constexpr int DT = DW * 32;
-  constexpr int KC = HD / 32;                    // 32-dim chunks of K
-  constexpr int VE = HD / 8 < 8 ? HD / 8 : 8;    // dims per V load
-  constexpr int VC = HD / (8 * VE);              // V loads per key
-  constexpr float RAISE = 4.f, BIAS = 11.f;
+  using C = MmaCfg<HD, DW>;
   using Smem = MmaSmem<HD, DW>;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  constexpr int DT = DW * 32, NB = C::HDP / 64, S = C::STAGES;
+  constexpr float RAISE = 4.f, BIAS = 11.f;
+  extern __shared__ uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const Work w = find_work<MMA_R>(p);
+  const int mine = (w.i1 - w.i0 - warp + DW - 1) / DW;  // pages of this warp (<= 0: none)
 
-  // page ids of this warp's entries i0 + warp + DW k, 32 at a time
-  int ids = 0, ids_at = 0;
+  // ids of this warp's entries i0 + warp + DW k, k = ids_at .. ids_at + 31; -1: outside the pool
+  int ids = -1, ids_at = 0;
   auto fetch_ids = [&](int k0) {
     const int i = w.i0 + warp + DW * (k0 + lane);
     ids = i < w.i1 ? page_id(p, w, i) : -1;
     ids_at = k0;
   };
-  const int mine = (w.i1 - w.i0 - warp + DW - 1) / DW;  // pages of this warp (<= 0: none)
-  if (mine > 0) fetch_ids(0);
-  const int64_t head_bytes = (int64_t)w.hk * PG * HD * 2, page_bytes = (int64_t)p.n_head_kv * PG * HD * 2;
-  // an id outside the pool reads page 0, and its keys count as masked
-  auto offset = [&](int k) { return (int64_t)max(__shfl_sync(0xffffffffu, ids, k - ids_at), 0) * page_bytes + head_bytes; };
-  uint32_t kr[KC][2][4], vr[4][VC][VE / 2];
-  auto load_k = [&](int64_t off) {
-    const uint8_t* b = static_cast<const uint8_t*>(p.k_pages) + off + g * (HD * 2) + t * 16;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      ldg_words(kr[c][0], b + c * 64);
-      ldg_words(kr[c][1], b + 8 * HD * 2 + c * 64);
+  uint8_t* slots = sm.ring + warp * S * 2 * C::PAGE;
+  // A page outside the pool comes as zeros (a row past the map's end); its keys count as masked.
+  auto issue = [&](int k) {
+    if (k - ids_at == 32) fetch_ids(k);
+    const int id = __shfl_sync(0xffffffffu, ids, k - ids_at);
+    if (lane == 0) {
+      const int y = id < 0 ? p.n_pages * p.n_head_kv * PG : (id * p.n_head_kv + w.hk) * PG;
+      uint64_t* bar = &sm.full[warp][k % S];
+      uint8_t* dst = slots + k % S * 2 * C::PAGE;
+      mbar_arrive_expect_tx(bar, 2 * C::PAGE);
+      tma_page(smem_u32(dst), &kmap, y, bar);
+      tma_page(smem_u32(dst + C::PAGE), &vmap, y, bar);
     }
+    return id;
   };
-  auto load_v = [&](int64_t off) {
-    const uint8_t* b = static_cast<const uint8_t*>(p.v_pages) + off + 2 * t * (HD * 2) + g * (VE * 2);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < VC; ++c) ldg_words(vr[j][c], b + ((j & 1) + (j & 2) * 4) * (HD * 2) + c * (16 * VE));
+  unsigned bad = 0;  // bit k % S: the page in that slot is outside the pool
+  auto issue_noting = [&](int k) {
+    const unsigned bit = 1u << (k % S);
+    bad = issue(k) < 0 ? bad | bit : bad & ~bit;
   };
-  // The next page's K is requested as soon as this page's is used up, its V
-  // likewise, so one of the two is always on its way.  At hd 256 the registers
-  // do not hold that: both are requested together when their page begins.
-  constexpr bool AHEAD = HD <= 128;
-  if (AHEAD && mine > 0) {
-    const int64_t off = offset(0);
-    load_k(off);
-    load_v(off);
+  if (lane == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&sm.full[warp][i], 1);
+    fence_mbar_init();
   }
+  __syncwarp();
+  if (mine > 0) fetch_ids(0);
+  for (int k = 0; k < min(mine, S); ++k) issue_noting(k);
 
-  // q as A operands: k-step s, lane (g, t): dims 32 (s / 2) + 8 t + 4 (s % 2) + 0..3
-  if (SPLIT && warp < MMA_R) {
+  // q as A operands: step 4 b + 2 h + u, lane (g, t): dims 64 b + 8 (2 t + h) + 4 u + 0..3 of head g
+  if (SPLIT) {
     for (int r = warp; r < MMA_R; r += DW) {
       float mx = 0.f;
       if (r < w.n_rows)
@@ -371,11 +389,12 @@ __global__ void __launch_bounds__(DW * 32, HD > 128 ? 8 / DW : 12 / DW)
     }
     __syncthreads();
   }
-  for (int i = tid; i < HD / 16 * 32; i += DT) {
+  for (int i = tid; i < C::HDP / 16 * 32; i += DT) {
     const int s = i / 32, gg = i % 32 / 4, tt = i % 4;
+    const int d = s / 4 * 64 + (2 * tt + s / 2 % 2) * 8 + s % 2 * 4;
     float x[4] = {};
-    if (gg < w.n_rows) {
-      const int64_t at = w.seq * p.q_stride + (int64_t)(w.head0 + gg) * HD + s / 2 * 32 + tt * 8 + s % 2 * 4;
+    if (gg < w.n_rows && d < HD) {
+      const int64_t at = w.seq * p.q_stride + (int64_t)(w.head0 + gg) * HD + d;
       const float down = SPLIT ? 1.f / sm.up[gg] : 1.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = load_elem(p.q, at + e, p.io) * down;
@@ -388,50 +407,43 @@ __global__ void __launch_bounds__(DW * 32, HD > 128 ? 8 / DW : 12 / DW)
   __syncthreads();
   const float scale = p.scale_log2 * (SPLIT ? sm.up[g] : 1.f);
 
-  float o[VC * VE][4];
+  float o[NB * 8][4];
 #pragma unroll
-  for (int i = 0; i < VC * VE; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < NB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m = -INFINITY, l = 0.f;  // of head g; l of this lane's keys
   for (int k = 0; k < mine; ++k) {
-    const int entry = w.i0 + warp + DW * k, j0 = w.sp.page(entry) * PG;
-    if (!AHEAD && k - ids_at == 32) fetch_ids(k);
-    const bool bad = __shfl_sync(0xffffffffu, ids, k - ids_at) < 0;
-    if (!AHEAD) {
-      const int64_t off = offset(k);
-      load_k(off);
-      load_v(off);
+    const int j0 = w.sp.page(w.i0 + warp + DW * k) * PG;
+    if (!wait_slot(&sm.full[warp][k % S], (uint32_t)(k / S) & 1, p.status)) {
+      const long long t0 = clock64();  // the copies still under way end before their memory is used again
+      while (clock64() - t0 < 1 << 20) {
+      }
+      break;
     }
+    const uint8_t* ks = slots + k % S * 2 * C::PAGE;
+    const uint8_t* vs = ks + C::PAGE;
     float s0[4] = {}, s1[4] = {};
 #pragma unroll
-    for (int c = 0; c < KC; ++c)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 q = sm.q[2 * c + h][lane];
-        const uint32_t a[4] = {q.x, q.y, q.z, q.w};
-        mma16816<BF16>(s0, a, kr[c][0][2 * h], kr[c][0][2 * h + 1]);
-        mma16816<BF16>(s1, a, kr[c][1][2 * h], kr[c][1][2 * h + 1]);
+        const uint8_t* at = ks + b * (PG * 128) + g * 128 + (((2 * t + h) ^ g) * 16);
+        const uint4 k0 = lds128(at), k1 = lds128(at + 8 * 128);
+        const uint4 qa = sm.q[4 * b + 2 * h][lane], qb = sm.q[4 * b + 2 * h + 1][lane];
+        const uint32_t a0[4] = {qa.x, qa.y, qa.z, qa.w}, a1[4] = {qb.x, qb.y, qb.z, qb.w};
+        mma16816<BF16>(s0, a0, k0.x, k0.y);
+        mma16816<BF16>(s1, a0, k1.x, k1.y);
+        mma16816<BF16>(s0, a1, k0.z, k0.w);
+        mma16816<BF16>(s1, a1, k1.z, k1.w);
       }
-    int64_t next = 0;
-    if (AHEAD && k + 1 < mine) {
-      if (k + 1 - ids_at == 32) fetch_ids(k + 1);
-      next = offset(k + 1);
-      load_k(next);
-    }
     // keys 2t, 2t+1, 2t+8, 2t+9 of head g
     float x[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
-    const bool edge = bad || j0 + PG - 1 > w.pos || (p.window > 0 && j0 <= w.pos - p.window);
-    if (edge) {
+    const bool gone = bad >> (k % S) & 1;
+    const bool edge = gone || j0 + PG - 1 > w.pos || (p.window > 0 && j0 <= w.pos - p.window);
+    bool see[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool see = !bad && key_seen(j0 + 2 * t + (j & 1) + (j & 2) * 4, w.pos, p.window, p.n_sink);
-        if (!see) {
-          x[j] = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < VC; ++c)  // whatever a masked place holds is not used
-#pragma unroll
-            for (int e = 0; e < VE / 2; ++e) vr[j][c][e] = 0;
-        }
-      }
+    for (int j = 0; j < 4; ++j) {
+      see[j] = !edge || (!gone && key_seen(j0 + 2 * t + (j & 1) + (j & 2) * 4, w.pos, p.window, p.n_sink));
+      if (!see[j]) x[j] = -INFINITY;
     }
     float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -442,7 +454,7 @@ __global__ void __launch_bounds__(DW * 32, HD > 128 ? 8 / DW : 12 / DW)
       m = mn;
       l *= f;
 #pragma unroll
-      for (int i = 0; i < VC * VE; ++i) {
+      for (int i = 0; i < NB * 8; ++i) {
         o[i][0] *= f;
         o[i][1] *= f;
         o[i][2] *= f;
@@ -457,34 +469,49 @@ __global__ void __launch_bounds__(DW * 32, HD > 128 ? 8 / DW : 12 / DW)
     two_terms<BF16>(x[0], x[1], a[0], a[1]);
     two_terms<BF16>(x[2], x[3], a[2], a[3]);
 #pragma unroll
-    for (int c = 0; c < VC; ++c)
+    for (int b = 0; b < NB; ++b) {
+      uint32_t v[4][4];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-        mma16816<BF16>(o[c * VE + e], a, __byte_perm(vr[0][c][e / 2], vr[1][c][e / 2], sel),
-                       __byte_perm(vr[2][c][e / 2], vr[3][c][e / 2], sel));
+      for (int j = 0; j < 4; ++j) {
+        const int key = 2 * t + (j & 1) + (j & 2) * 4;
+        const uint4 r = lds128(vs + b * (PG * 128) + key * 128 + ((g ^ (key & 7)) * 16));
+        // whatever a masked place holds is not used
+        v[j][0] = see[j] ? r.x : 0;
+        v[j][1] = see[j] ? r.y : 0;
+        v[j][2] = see[j] ? r.z : 0;
+        v[j][3] = see[j] ? r.w : 0;
       }
-    if (AHEAD && k + 1 < mine) load_v(next);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+        mma16816<BF16>(o[b * 8 + e], a, __byte_perm(v[0][e / 2], v[1][e / 2], sel),
+                       __byte_perm(v[2][e / 2], v[3][e / 2], sel));
+      }
+    }
+    __syncwarp();  // every lane is done with the slot
+    if (k + S < mine) issue_noting(k + S);
   }
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
+  __syncthreads();  // the ring becomes the join's memory
   if (t == 0) {
     sm.join.m[warp][g] = m;
     sm.join.l[warp][g] = l;
   }
 #pragma unroll
-  for (int c = 0; c < VC; ++c)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      float* dst = &sm.join.o[warp][g][c * 8 * VE + 2 * t * VE + e];
-      dst[0] = o[c * VE + e][0] + o[c * VE + e][2];
-      dst[VE] = o[c * VE + e][1] + o[c * VE + e][3];
+    for (int e = 0; e < 8; ++e) {
+      const int d = b * 64 + 16 * t + e;  // and d + 8
+      if (d < HD) sm.join.o[warp][g][d] = o[b * 8 + e][0] + o[b * 8 + e][2];
+      if (d + 8 < HD) sm.join.o[warp][g][d + 8] = o[b * 8 + e][1] + o[b * 8 + e][3];
     }
   join_and_store(sm.join, p, w.seq, w.head0, w.n_rows, w.pos >= 0);
 }
 
-template <class K>
-cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st) {
+template <class K, class... Maps>
+cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st,
+                            const Maps&... maps) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   if (p.cluster > 8) {
@@ -502,7 +529,7 @@ cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, int 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p, maps...);
 }
 
 // pages that the longest possible context of this call sees
@@ -529,28 +556,35 @@ cudaError_t launch_cc(WindowAttnParams& p, int sm_count, cudaStream_t st) {
 }
 
 template <class KV, int HD, bool SPLIT, int DW>
-cudaError_t launch_mma(WindowAttnParams& p, int tiles, cudaStream_t st) {
-  return launch_clusters(decode_mma_kernel<KV, HD, SPLIT, DW>, p, tiles, DW * 32, sizeof(MmaSmem<HD, DW>), st);
+cudaError_t launch_mma(WindowAttnParams& p, int kv, int tiles, cudaStream_t st) {
+  CUtensorMap km, vm;
+  const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
+  cudaError_t e = pool_map(&km, p.k_pages, kv, HD, rows, (HD + 63) / 64);
+  if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, (HD + 63) / 64);
+  if (e != cudaSuccess) return e;
+  return launch_clusters(decode_mma_kernel<KV, HD, SPLIT, DW>, p, tiles, DW * 32, sizeof(MmaSmem<HD, DW>) + 1024, st, km, vm);
 }
 template <class KV, int HD>
-cudaError_t launch_16(WindowAttnParams& p, int sm_count, cudaStream_t st) {
+cudaError_t launch_16(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
+  if ((int64_t)p.n_pages * p.n_head_kv * PG >= 0x7fffffff) return launch_cc<KV, HD>(p, sm_count, st);  // beyond a map's rows
   const int tiles = (p.n_head / p.n_head_kv + MMA_R - 1) / MMA_R;
   const bool split = p.io == EL_F32;
-  // Two or more CTAs of four warps for every SM if the batch gives them, else CTAs of eight warps
-  p.cluster = pick_cluster(p, tiles, 4, 3 * sm_count);
+  // Two CTAs of four warps for every SM if the batch gives them, else one CTA of eight warps
+  p.cluster = pick_cluster(p, tiles, 4, 2 * sm_count);
   const int64_t ctas = (int64_t)p.n_seq * p.n_head_kv * tiles * p.cluster;
-  if (ctas >= 2 * sm_count || max_seen_pages(p) < p.cluster * 8)
-    return split ? launch_mma<KV, HD, true, 4>(p, tiles, st) : launch_mma<KV, HD, false, 4>(p, tiles, st);
-  return split ? launch_mma<KV, HD, true, 8>(p, tiles, st) : launch_mma<KV, HD, false, 8>(p, tiles, st);
+  if constexpr (HD <= 128)
+    if (ctas < 2 * sm_count && max_seen_pages(p) >= p.cluster * 8)
+      return split ? launch_mma<KV, HD, true, 8>(p, kv, tiles, st) : launch_mma<KV, HD, false, 8>(p, kv, tiles, st);
+  return split ? launch_mma<KV, HD, true, 4>(p, kv, tiles, st) : launch_mma<KV, HD, false, 4>(p, kv, tiles, st);
 }
 
 template <int HD>
 cudaError_t launch_hd(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
   if (kv == EL_F32) return launch_cc<float, HD>(p, sm_count, st);
-  if (kv == EL_F16) return launch_16<__half, HD>(p, sm_count, st);
+  if (kv == EL_F16) return launch_16<__half, HD>(p, kv, sm_count, st);
   // 32-bit rows over a bf16 cache: two bf16 terms hold 16 bits only, so these stay on the CUDA cores
   if (p.io == EL_F32) return launch_cc<__nv_bfloat16, HD>(p, sm_count, st);
-  return launch_16<__nv_bfloat16, HD>(p, sm_count, st);
+  return launch_16<__nv_bfloat16, HD>(p, kv, sm_count, st);
 }
 
 }  // namespace

@@ -33,11 +33,10 @@
 // memory; a V row that some rows of a tile see and others do not reaches the
 // others as 0 * v, which is NaN for an infinite v: rows whose output is not
 // finite are computed again key by key (recompute_row).
-#include <cuda.h>
-
 #include <type_traits>
 
 #include "sfk_paged.cuh"
+#include "sfk_paged_map.cuh"
 
 namespace sfk {
 namespace {
@@ -175,15 +174,6 @@ __host__ __device__ constexpr uint32_t idesc_f16(int bf16, int n, int b_mn) {
   return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 |
          (uint32_t)(TM >> 4) << 24;
 }
-// 16 rows x 64 elements of the map at (column x, row y)
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -512,7 +502,7 @@ __global__ void __launch_bounds__(TT, 1)
         const uint32_t dst = smem_u32(ring + slot * C::TILE);
         const int yy = __shfl_sync(0xffffffffu, y, lane % PPT);
         if (lane < PPT * C::HALVES)
-          tma_2d(dst + (lane / PPT) * (TK * 128) + (lane % PPT) * (PG * 128), v ? &vmap : &kmap, lane / PPT * 64, yy, bar);
+          tma_page(dst + (lane / PPT) * (TK * 128) + (lane % PPT) * (PG * 128), v ? &vmap : &kmap, yy, bar, lane / PPT);
         __syncwarp();
         if (fix) {
           ok = wait_warp(&c->tail, 0, c, p.status);
@@ -602,41 +592,13 @@ __global__ void __launch_bounds__(TT, 1)
 }
 
 // ---- host -----------------------------------------------------------------------------------
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<EncodeTiled>(f);
-  }();
-  return fn;
-}
-
-// the pool as a matrix of its [n_pages * Hkv * 16] rows of hd elements; a copy takes one page's 16 rows, 64 columns
-cudaError_t pool_map(CUtensorMap* m, const void* pool, int kv, int hd, int64_t rows) {
-  const EncodeTiled fn = encode_tiled();
-  if (!fn) return cudaErrorNotSupported;
-  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
-  const cuuint32_t box[2] = {64, PG}, step[2] = {1, 1};
-  return fn(m, kv == EL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-            const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-             ? cudaSuccess
-             : cudaErrorInvalidValue;
-}
-
 template <class KV, int HD, bool SPLIT>
 cudaError_t launch_t(WindowAttnParams& p, int kv, cudaStream_t st) {
   using C = Cfg<HD, SPLIT>;
   CUtensorMap km, vm;
   const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
-  cudaError_t e = pool_map(&km, p.k_pages, kv, HD, rows);
-  if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows);
+  cudaError_t e = pool_map(&km, p.k_pages, kv, HD, rows, 1);
+  if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, 1);
   if (e != cudaSuccess) return e;
   const auto kernel = prefill_tc_kernel<KV, HD, SPLIT>;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
