@@ -512,8 +512,8 @@ SFK_API sfk_status sfk_attn_decode_paged(const float *dev_q, const void *dev_k_p
  *     row.
  *   - A call launches on `stream` (of the current device, where the pointers
  *     live) and returns without waiting.  It allocates nothing and keeps
- *     nothing: calls on several streams are independent, and all three can be
- *     captured into CUDA graphs.
+ *     nothing: calls on several streams are independent (each with a workspace
+ *     of its own), and all three can be captured into CUDA graphs.
  *   - dev_status (optional): one device int32, zero before the first call.  A
  *     position, length, sequence or page id outside its range is never
  *     dereferenced; it stores a code there, and sfk_device_status (which waits
@@ -550,13 +550,21 @@ SFK_API sfk_status sfk_qk_norm_rope_append(
  * j > p - window or j < n_sink.  scale 0: 1 / sqrt(head_dim).  A negative
  * position is a padding row and gives zeros.  head_dim 32, 64, 128 or 256; any
  * number of query heads per kv head; 16-bit rows need a cache of their own
- * type, f32 rows take any.  out: [n_seq][n_head * head_dim]. */
+ * type, f32 rows take any.  out: [n_seq][n_head * head_dim].
+ * dev_workspace (optional, 16-byte aligned device memory) belongs to the call
+ * until its work is done and holds nothing between calls; with less than
+ * sfk_attn_decode_window_workspace bytes, or none, a small batch over a long
+ * context is split over fewer CTAs. */
 SFK_API sfk_status sfk_attn_decode_window(int32_t io_type, const void *dev_q, int64_t q_stride, int32_t kv_type,
                                           const void *dev_k_pages, const void *dev_v_pages, int32_t n_pages,
                                           const int32_t *dev_page_table, int32_t max_pages, const int32_t *dev_positions,
                                           int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
                                           float scale, int32_t window, int32_t n_sink, void *dev_out,
-                                          int32_t *dev_status, void *stream);
+                                          void *dev_workspace, size_t workspace_bytes, int32_t *dev_status,
+                                          void *stream);
+/* Bytes of workspace with which that call is fastest (0: it uses none; it
+ * depends on the sizes and the current device alone). */
+SFK_API size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t head_dim);
 
 /* The same attention for the newest tokens of each of n_seq sequences: rows
  * q_start[s] .. q_start[s+1]-1 of q (q_start [n_seq + 1], ascending, device)

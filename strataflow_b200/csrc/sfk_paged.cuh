@@ -64,13 +64,17 @@ struct WindowAttnParams {
   // decode
   const int* pos;    // [n_seq]
   int n_seq;
-  int cluster;       // CTAs that share one (sequence, kv head, row tile)
+  int parts;         // CTAs that share one (sequence, kv head, row tile)
+  float* partial;    // where they join: null, a cluster; else this workspace
+  size_t ws_bytes;
   // prefill
   const int* q_start;  // [n_seq + 1]
   const int* kv_len;   // [n_seq]
   int n_tok;
 };
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
+// p.partial / p.ws_bytes: the caller's workspace, or null
+size_t window_decode_workspace(int64_t n_seq, int n_head, int n_head_kv, int hd, int sm_count);
 cudaError_t launch_window_prefill(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
 // the tensor-core form: whether it takes these types and sizes, and its launch
 bool prefill_tc_takes(const WindowAttnParams& p, int kv, int hd);

@@ -158,7 +158,8 @@ sfk_status sfk_qk_norm_rope_append(int32_t io_type, const void* q, int64_t q_str
 sfk_status sfk_attn_decode_window(int32_t io_type, const void* q, int64_t q_stride, int32_t kv_type, const void* kp,
                                   const void* vp, int32_t n_pages, const int32_t* table, int32_t max_pages,
                                   const int32_t* positions, int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t hd,
-                                  float scale, int32_t window, int32_t n_sink, void* out, int32_t* status, void* stream) {
+                                  float scale, int32_t window, int32_t n_sink, void* out, void* workspace,
+                                  size_t workspace_bytes, int32_t* status, void* stream) {
   const char* who = "attn_decode_window";
   if (n_seq < 0 || n_seq > 65535) BAD("%s: %d sequences (at most 65535)", who, n_seq);
   if (n_seq == 0) return SFK_OK;
@@ -168,10 +169,18 @@ sfk_status sfk_attn_decode_window(int32_t io_type, const void* q, int64_t q_stri
                                n_head_kv, hd, scale, window, n_sink, out))
     return s;
   if (!positions) BAD("%s: null pointer", who);
+  if (!aligned16(workspace)) BAD("%s: the workspace starts on a 16-byte boundary", who);
+  a.partial = static_cast<float*>(workspace);
+  a.ws_bytes = workspace ? workspace_bytes : 0;
   a.pos = positions;
   a.n_seq = n_seq;
   a.status = status;
   return cuda_result(launch_window_decode(a, kv, hd, current_sms(), (cudaStream_t)stream), who);
+}
+
+size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t hd) {
+  if (n_seq < 1 || n_head < 1 || n_head_kv < 1 || n_head % n_head_kv || hd < 1 || hd > 256) return 0;
+  return window_decode_workspace(n_seq, n_head, n_head_kv, hd, current_sms());
 }
 
 sfk_status sfk_attn_prefill_window(int32_t io_type, const void* q, int64_t q_stride, int32_t n_tok, int32_t kv_type,

@@ -1,16 +1,19 @@
 // sfk_paged_decode.cu -- attention of one new token of each sequence over the
 // keys it sees in the paged cache (window and sinks), split over the keys and
-// joined inside a thread-block cluster.
+// joined.
 //
 //   s_j = scale q . k_j  for the seen keys j;  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
 //
 // Bound by memory: each seen key and value is read once for all query heads
-// of its kv head.  A cluster takes one (sequence, kv head); each CTA takes a
-// run of its seen pages, each warp every W-th page of the run with a running
-// maximum, sum and output of its own (f32).  The partials of the warps meet in
-// shared memory, those of the CTAs in distributed shared memory: no scratch
-// in global memory, no second launch, and calls on several streams or in
-// several graphs have nothing in common.
+// of its kv head.  The seen pages of one (sequence, kv head, 8 query heads) are
+// split over CTAs; each warp takes every W-th page of its CTA's run with a
+// running maximum, sum and output of its own (f32).  The partials of the warps
+// meet in shared memory, those of the CTAs
+//   - in the distributed shared memory of a cluster of up to 8 (no scratch, one
+//     launch), or,
+//   - where the batch is too small for such clusters to fill the GPU, in the
+//     caller's workspace, joined by a second kernel that is already resident when
+//     the first ends.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -36,6 +39,77 @@ __device__ __forceinline__ bool wait_slot(uint64_t* bar, uint32_t parity, int* s
   return __all_sync(0xffffffffu, ok);
 }
 
+// The workspace: o [n_seq * n_head][parts][HD], then (m, l) [n_seq * n_head][parts]
+template <int HD>
+__device__ __forceinline__ float* partial_o(const WindowAttnParams& p, int seq, int head, int part) {
+  return p.partial + (((int64_t)seq * p.n_head + head) * p.parts + part) * HD;
+}
+template <int HD>
+__device__ __forceinline__ float2* partial_ml(const WindowAttnParams& p, int seq, int head, int part) {
+  return reinterpret_cast<float2*>(p.partial + (int64_t)p.n_seq * p.n_head * p.parts * HD) +
+         ((int64_t)seq * p.n_head + head) * p.parts + part;
+}
+// One query head: warp w adds parts w, w + 8, ..., the warps meet in shared memory
+// (a fixed order: the same bits each time).  Launched while the parts are
+// computed (programmatic dependent launch); waits for all of them.
+constexpr int JW = 8;  // warps
+template <int HD>
+__global__ void __launch_bounds__(JW * 32) join_kernel(const __grid_constant__ WindowAttnParams p) {
+  constexpr int E = HD / 32;
+  extern __shared__ float weight[];  // [parts]
+  __shared__ float red[JW], lsum[JW], os[JW][HD];
+  const int seq = blockIdx.x / p.n_head, head = blockIdx.x % p.n_head;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int pos = p.pos[seq];
+  pdl_wait();
+  const float2* ml = partial_ml<HD>(p, seq, head, 0);
+  const float* po = partial_o<HD>(p, seq, head, 0) + lane * E;
+  float m = -INFINITY;
+  for (int c = tid; c < p.parts; c += JW * 32) m = fmaxf(m, ml[c].x);
+  m = warp_max(m);
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JW; ++w) m = fmaxf(m, red[w]);
+  if (m == -INFINITY) m = 0.f;
+  float l = 0.f;
+  for (int c = tid; c < p.parts; c += JW * 32) {
+    const float2 x = ml[c];
+    const float f = exp2_approx(x.x - m);
+    weight[c] = f;
+    l += x.y * f;
+  }
+  l = warp_sum(l);
+  if (lane == 0) lsum[warp] = l;
+  __syncthreads();
+  float o[E] = {};
+#pragma unroll 4
+  for (int c = warp; c < p.parts; c += JW) {
+    float x[E];
+    if constexpr (E % 4 == 0) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(x + e) = *reinterpret_cast<const float4*>(po + (int64_t)c * HD + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = po[(int64_t)c * HD + e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(x[e], weight[c], o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) os[warp][lane * E + e] = o[e];
+  __syncthreads();
+  if (tid < HD) {
+    float sum = 0.f, ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < JW; ++w) {
+      sum += os[w][tid];
+      ls += lsum[w];
+    }
+    store_elem(p.out, ((int64_t)seq * p.n_head + head) * HD + tid, pos >= 0 && pos / PG < p.max_pages ? sum / ls : 0.f, p.io);
+  }
+}
+
 // ---- join -----------------------------------------------------------------------
 // Every warp's partial (m, l, o) of R rows to the output.  m is in units of
 // log2; a partial without keys has m = -inf, l = 0, o = 0.
@@ -51,7 +125,7 @@ template <int R, int HD, int DW>
 __device__ void join_and_store(JoinSmem<R, HD, DW>& sm, const WindowAttnParams& p, int seq, int head0, int n_rows, bool any) {
   constexpr int DT = DW * 32;
   cg::cluster_group cl = cg::this_cluster();
-  const int C = p.cluster, rank = C > 1 ? (int)cl.block_rank() : 0;
+  const int C = p.partial ? 1 : p.parts, rank = C > 1 ? (int)cl.block_rank() : 0;
   const int tid = threadIdx.x;
   __syncthreads();
   if (tid < R) {
@@ -72,7 +146,12 @@ __device__ void join_and_store(JoinSmem<R, HD, DW>& sm, const WindowAttnParams& 
     const int r = i / HD, d = i % HD;
     float o = 0.f;
     for (int w = 0; w < DW; ++w) o += sm.o[w][r][d] * sm.m[w][r];
-    sm.co[r][d] = o;
+    if (p.partial) partial_o<HD>(p, seq, head0 + r, blockIdx.x % p.parts)[d] = o;
+    else sm.co[r][d] = o;
+  }
+  if (p.partial) {
+    if (tid < n_rows) *partial_ml<HD>(p, seq, head0 + tid, blockIdx.x % p.parts) = make_float2(sm.cm[tid], sm.cl[tid]);
+    return;
   }
   if (C > 1) cl.sync();
   else __syncthreads();
@@ -111,8 +190,8 @@ template <int R>
 __device__ __forceinline__ Work find_work(const WindowAttnParams& p) {
   Work w;
   const int group = p.n_head / p.n_head_kv, tiles = (group + R - 1) / R;
-  const int rank = blockIdx.x % p.cluster;
-  const int pair = blockIdx.x / p.cluster;
+  const int rank = blockIdx.x % p.parts;
+  const int pair = blockIdx.x / p.parts;
   w.hk = pair / tiles;
   const int tile = pair % tiles;
   w.head0 = w.hk * group + tile * R;
@@ -125,9 +204,9 @@ __device__ __forceinline__ Work find_work(const WindowAttnParams& p) {
     w.pos = -1;
   }
   if (w.pos >= 0) w.sp = seen_pages(w.pos, w.pos, p.window, p.n_sink);
-  const int per = (w.sp.n + p.cluster - 1) / p.cluster;
-  w.i0 = min(w.sp.n, rank * per);
-  w.i1 = min(w.sp.n, w.i0 + per);
+  // runs that differ by a page at most
+  w.i0 = (int)((int64_t)w.sp.n * rank / p.parts);
+  w.i1 = (int)((int64_t)w.sp.n * (rank + 1) / p.parts);
   return w;
 }
 // the page id of list entry i, or -1
@@ -157,6 +236,7 @@ __global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(cons
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  if (p.partial) pdl_launch_dependents();
   const Work w = find_work<R>(p);
   for (int i = tid; i < R * HD; i += DT) {
     const int r = i / HD;
@@ -309,8 +389,7 @@ template <int HD, int DW>
 struct MmaCfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;    // head width in a slot (the copy fills with zeros)
   static constexpr int PAGE = PG * HDP * 2;        // bytes of a page's K or V
-  static constexpr int FIT = 96 * 1024 / (4 * 2 * PAGE);
-  static constexpr int STAGES = FIT < 3 ? 3 : FIT; // slots per warp: 24 KB of copies under way, or three pages
+  static constexpr int STAGES = HDP == 64 ? 4 : 2;  // slots per warp: 16 KB (32 KB at hd 256)
   static constexpr int RING = DW * STAGES * 2 * PAGE;
 };
 template <int HD, int DW>
@@ -326,7 +405,7 @@ struct MmaSmem {
 };
 
 template <class KV, int HD, bool SPLIT, int DW>
-__global__ void __launch_bounds__(DW * 32, HD <= 128 && DW == 4 ? 2 : 1)
+__global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
     decode_mma_kernel(const __grid_constant__ WindowAttnParams p, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap) {
   constexpr bool BF16 = std::is_same<KV, __nv_bfloat16>::value;
@@ -337,6 +416,31 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 && DW == 4 ? 2 : 1)
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  static_assert(DT == MMA_R * 16, "16 threads to a query head");
+  if (p.partial) pdl_launch_dependents();
+  if (tid == 0) {
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
+  }
+  // q is on its way while the position and the page ids are looked up
+  constexpr int QC = (C::HDP / 8 + 15) / 16;
+  const int qr = tid / 16, qi = tid % 16;
+  float qx[QC][8] = {};
+  {
+    const int group = p.n_head / p.n_head_kv, tiles = (group + MMA_R - 1) / MMA_R, pair = blockIdx.x / p.parts;
+    const int r = pair % tiles * MMA_R + qr;
+    if (r < group) {
+      const int64_t at = blockIdx.y * p.q_stride + (int64_t)(pair / tiles * group + r) * HD;
+#pragma unroll
+      for (int c = 0; c < QC; ++c)
+        if ((qi + 16 * c) * 8 < HD) {
+          using Row = typename std::conditional<SPLIT, float, KV>::type;
+          Raw8<Row> raw;
+          load8(raw, static_cast<const Row*>(p.q) + at + (qi + 16 * c) * 8, p.q_vec);
+          unpack8(raw, qx[c]);
+        }
+    }
+  }
   const Work w = find_work<MMA_R>(p);
   const int mine = (w.i1 - w.i0 - warp + DW - 1) / DW;  // pages of this warp (<= 0: none)
 
@@ -376,33 +480,32 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 && DW == 4 ? 2 : 1)
   for (int k = 0; k < min(mine, S); ++k) issue_noting(k);
 
   // q as A operands: step 4 b + 2 h + u, lane (g, t): dims 64 b + 8 (2 t + h) + 4 u + 0..3 of head g
+  float mx = 0.f;
+#pragma unroll
+  for (int c = 0; c < QC; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(qx[c][e]));
+  float up = 1.f;  // the head's largest |q| to [1, 2): a power of two, exact
   if (SPLIT) {
-    for (int r = warp; r < MMA_R; r += DW) {
-      float mx = 0.f;
-      if (r < w.n_rows)
-        for (int d = lane; d < HD; d += 32)
-          mx = fmaxf(mx, fabsf(load_elem(p.q, w.seq * p.q_stride + (int64_t)(w.head0 + r) * HD + d, p.io)));
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-      const int e = (int)(__float_as_uint(mx) >> 23) - 127;  // largest |q| to [1, 2): exact
-      if (lane == 0) sm.up[r] = mx > 0.f && e < 128 ? exp2f((float)max(e, -126)) : 1.f;
-    }
-    __syncthreads();
+    for (int d = 1; d < 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const int e = (int)(__float_as_uint(mx) >> 23) - 127;
+    if (mx > 0.f && e < 128) up = __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
+    if (qi == 0) sm.up[qr] = up;
   }
-  for (int i = tid; i < C::HDP / 16 * 32; i += DT) {
-    const int s = i / 32, gg = i % 32 / 4, tt = i % 4;
-    const int d = s / 4 * 64 + (2 * tt + s / 2 % 2) * 8 + s % 2 * 4;
-    float x[4] = {};
-    if (gg < w.n_rows && d < HD) {
-      const int64_t at = w.seq * p.q_stride + (int64_t)(w.head0 + gg) * HD + d;
-      const float down = SPLIT ? 1.f / sm.up[gg] : 1.f;
+  const float down = 1.f / up;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = load_elem(p.q, at + e, p.io) * down;
+  for (int c = 0; c < QC; ++c) {
+    const int ch = qi + 16 * c;  // 8 dims
+    if (ch < C::HDP / 8) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint4 a;
+        two_terms<BF16>(qx[c][4 * u] * down, qx[c][4 * u + 1] * down, a.x, a.y);  // 16-bit rows: the second term is 0
+        two_terms<BF16>(qx[c][4 * u + 2] * down, qx[c][4 * u + 3] * down, a.z, a.w);
+        sm.q[ch / 8 * 4 + ch % 2 * 2 + u][qr * 4 + ch % 8 / 2] = a;
+      }
     }
-    uint4 a;
-    two_terms<BF16>(x[0], x[1], a.x, a.y);  // 16-bit rows: the second term is 0
-    two_terms<BF16>(x[2], x[3], a.z, a.w);
-    sm.q[s][i % 32] = a;
   }
   __syncthreads();
   const float scale = p.scale_log2 * (SPLIT ? sm.up[g] : 1.f);
@@ -510,26 +613,37 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 && DW == 4 ? 2 : 1)
 }
 
 template <class K, class... Maps>
-cudaError_t launch_clusters(K kernel, const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st,
-                            const Maps&... maps) {
+cudaError_t launch_parts(K kernel, const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st,
+                         const Maps&... maps) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  if (p.cluster > 8) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.n_head_kv * tiles * p.cluster), (unsigned)p.n_seq);
+  cfg.gridDim = dim3((unsigned)(p.n_head_kv * tiles * p.parts), (unsigned)p.n_seq);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)p.cluster;
+  attr.val.clusterDim.x = (unsigned)(p.partial ? 1 : p.parts);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, p, maps...);
+}
+
+template <int HD>
+cudaError_t launch_join(const WindowAttnParams& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.n_seq * p.n_head));
+  cfg.blockDim = dim3(JW * 32);
+  cfg.dynamicSmemBytes = sizeof(float) * p.parts;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<HD>, p);
 }
 
 // pages that the longest possible context of this call sees
@@ -538,56 +652,75 @@ int64_t max_seen_pages(const WindowAttnParams& p) {
   const int64_t n = (p.window + (int64_t)PG - 1) / PG + 1 + ((int64_t)p.n_sink + PG - 1) / PG;
   return n < p.max_pages ? n : p.max_pages;
 }
-// CTAs per (sequence, kv head, row tile): enough for `want` in all, as long as
-// each warp has a page or more.
-int pick_cluster(const WindowAttnParams& p, int tiles, int warps, int64_t want) {
-  const int64_t pages = max_seen_pages(p), pairs = (int64_t)p.n_seq * p.n_head_kv * tiles;
+
+constexpr int DEC_R = 8, DEC_W = 4;  // query heads and warps of a CTA
+int row_tiles(const WindowAttnParams& p) { return (p.n_head / p.n_head_kv + DEC_R - 1) / DEC_R; }
+
+// How many CTAs share a (sequence, kv head, row tile), and where they join.
+// Short contexts: a cluster of up to 8, doubled until the GPU has two CTAs for
+// every SM, as long as each warp keeps a page or more.  Where a warp would still
+// walk more than LONG pages that way, the pages are split into one wave of `occ`
+// CTAs per SM, joined through the workspace.
+constexpr int LONG = 2;
+void pick_parts(WindowAttnParams& p, int occ, int hd, int sm_count) {
+  const int64_t pages = max_seen_pages(p), pairs = (int64_t)p.n_seq * p.n_head_kv * row_tiles(p);
   int c = 1;
-  while (c < 16 && pairs * c < want && pages > (int64_t)c * warps) c *= 2;
-  return c;
+  while (c < 8 && pairs * c < 2 * sm_count && pages > (int64_t)c * DEC_W) c *= 2;
+  p.parts = c;
+  float* ws = p.partial;
+  p.partial = nullptr;
+  int64_t n = occ * sm_count / pairs;
+  n = n < pages / (2 * DEC_W) ? n : pages / (2 * DEC_W);
+  if (n > 1 && pages > (int64_t)c * DEC_W * LONG && ws &&
+      p.ws_bytes >= (size_t)(n * p.n_seq * p.n_head * (hd + 2)) * sizeof(float)) {
+    p.parts = (int)n;
+    p.partial = ws;
+  }
 }
 
 template <class KV, int HD>
 cudaError_t launch_cc(WindowAttnParams& p, int sm_count, cudaStream_t st) {
   using Smem = CcSmem<KV, HD>;
-  const int tiles = (p.n_head / p.n_head_kv + Smem::R - 1) / Smem::R;
-  p.cluster = pick_cluster(p, tiles, Smem::DW, 2 * sm_count);
-  return launch_clusters(decode_cc_kernel<KV, HD>, p, tiles, Smem::DW * 32, sizeof(Smem), st);
+  static_assert(Smem::R == DEC_R && Smem::DW == DEC_W, "pick_parts counts these");
+  pick_parts(p, 2, HD, sm_count);
+  return launch_parts(decode_cc_kernel<KV, HD>, p, row_tiles(p), DEC_W * 32, sizeof(Smem), st);
 }
 
-template <class KV, int HD, bool SPLIT, int DW>
-cudaError_t launch_mma(WindowAttnParams& p, int kv, int tiles, cudaStream_t st) {
+template <class KV, int HD, bool SPLIT>
+cudaError_t launch_mma(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
+  using Smem = MmaSmem<HD, DEC_W>;
   CUtensorMap km, vm;
   const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
   cudaError_t e = pool_map(&km, p.k_pages, kv, HD, rows, (HD + 63) / 64);
   if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, (HD + 63) / 64);
   if (e != cudaSuccess) return e;
-  return launch_clusters(decode_mma_kernel<KV, HD, SPLIT, DW>, p, tiles, DW * 32, sizeof(MmaSmem<HD, DW>) + 1024, st, km, vm);
+  pick_parts(p, HD <= 128 ? 3 : 1, HD, sm_count);
+  return launch_parts(decode_mma_kernel<KV, HD, SPLIT, DEC_W>, p, row_tiles(p), DEC_W * 32, sizeof(Smem) + 1024, st, km, vm);
 }
 template <class KV, int HD>
 cudaError_t launch_16(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
   if ((int64_t)p.n_pages * p.n_head_kv * PG >= 0x7fffffff) return launch_cc<KV, HD>(p, sm_count, st);  // beyond a map's rows
-  const int tiles = (p.n_head / p.n_head_kv + MMA_R - 1) / MMA_R;
-  const bool split = p.io == EL_F32;
-  // Two CTAs of four warps for every SM if the batch gives them, else one CTA of eight warps
-  p.cluster = pick_cluster(p, tiles, 4, 2 * sm_count);
-  const int64_t ctas = (int64_t)p.n_seq * p.n_head_kv * tiles * p.cluster;
-  if constexpr (HD <= 128)
-    if (ctas < 2 * sm_count && max_seen_pages(p) >= p.cluster * 8)
-      return split ? launch_mma<KV, HD, true, 8>(p, kv, tiles, st) : launch_mma<KV, HD, false, 8>(p, kv, tiles, st);
-  return split ? launch_mma<KV, HD, true, 4>(p, kv, tiles, st) : launch_mma<KV, HD, false, 4>(p, kv, tiles, st);
+  return p.io == EL_F32 ? launch_mma<KV, HD, true>(p, kv, sm_count, st) : launch_mma<KV, HD, false>(p, kv, sm_count, st);
 }
 
 template <int HD>
 cudaError_t launch_hd(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
-  if (kv == EL_F32) return launch_cc<float, HD>(p, sm_count, st);
-  if (kv == EL_F16) return launch_16<__half, HD>(p, kv, sm_count, st);
+  cudaError_t e;
+  if (kv == EL_F32) e = launch_cc<float, HD>(p, sm_count, st);
+  else if (kv == EL_F16) e = launch_16<__half, HD>(p, kv, sm_count, st);
   // 32-bit rows over a bf16 cache: two bf16 terms hold 16 bits only, so these stay on the CUDA cores
-  if (p.io == EL_F32) return launch_cc<__nv_bfloat16, HD>(p, sm_count, st);
-  return launch_16<__nv_bfloat16, HD>(p, kv, sm_count, st);
+  else if (p.io == EL_F32) e = launch_cc<__nv_bfloat16, HD>(p, sm_count, st);
+  else e = launch_16<__nv_bfloat16, HD>(p, kv, sm_count, st);
+  return e == cudaSuccess && p.partial ? launch_join<HD>(p, st) : e;
 }
 
 }  // namespace
+
+size_t window_decode_workspace(int64_t n_seq, int n_head, int n_head_kv, int hd, int sm_count) {
+  // at most three CTAs for every SM write 8 heads each; none where one for each part of the batch fills that
+  const int64_t pairs = n_seq * n_head_kv * ((n_head / n_head_kv + DEC_R - 1) / DEC_R);
+  return pairs * 2 <= 3 * sm_count ? (size_t)3 * sm_count * DEC_R * (hd + 2) * sizeof(float) : 0;
+}
 
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {
   switch (hd) {

@@ -21,6 +21,9 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
       "l"(map), "r"(0), "r"(y), "r"(block), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 #endif
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -9,6 +9,7 @@ current CUDA stream.  Mirrors the ggml ops the reference's decode path issues
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -290,6 +291,12 @@ def _attn_rows(q: torch.Tensor, k_pages: torch.Tensor, kvh: int, hd: int, window
     return heads, qp, qs, out
 
 
+@functools.lru_cache(maxsize=4096)
+def _decode_workspace(n_seq: int, heads: int, kvh: int, hd: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return int(L.load().sfk_attn_decode_window_workspace(n_seq, heads, kvh, hd))
+
+
 def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                        positions: torch.Tensor, *, window: int = 0, n_sink: int = 0, scale: float = 0.0,
                        out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
@@ -300,10 +307,12 @@ def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
     heads, qp, qs, out = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
     n = q.shape[0]
+    ws_bytes = _decode_workspace(n, heads, kvh, hd, dev.index)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _call(dev, L.load().sfk_attn_decode_window, _ROW_TYPES[q.dtype], qp, qs, kvt, k_pages.data_ptr(),
           v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
           page_table.shape[1], _int32(positions, "positions", (n,), dev), n, heads, kvh, hd, scale, window, n_sink,
-          out.data_ptr(), _status(status, dev))
+          out.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _status(status, dev))
     return out
 
 

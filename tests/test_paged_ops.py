@@ -21,7 +21,7 @@ APPEND = dict(io=L.TYPE_F32, q=X, qs=8 * 64, k=X, ks=2 * 64, v=X, vs=2 * 64, n=3
               eps=1e-6, neox=0, n_rot=64, freqs=X, rope_pos=None, n_axes=0, axis=None, kvt=L.KV_F16, kp=X, vp=X,
               n_pages=4, table=X, n_seq=3, max_pages=2, seq=None, pos=X, out=X, outs=8 * 64, status=None, stream=None)
 DECODE = dict(io=L.TYPE_F32, q=X, qs=8 * 64, kvt=L.KV_F16, kp=X, vp=X, n_pages=4, table=X, max_pages=2, pos=X, n=3, hq=8,
-              hkv=2, hd=64, scale=0.0, window=0, sink=0, out=X, status=None, stream=None)
+              hkv=2, hd=64, scale=0.0, window=0, sink=0, out=X, ws=None, ws_bytes=0, status=None, stream=None)
 PREFILL = dict(io=L.TYPE_F32, q=X, qs=8 * 64, n_tok=5, kvt=L.KV_F16, kp=X, vp=X, n_pages=4, table=X, max_pages=2, start=X,
                lens=X, n=3, hq=8, hkv=2, hd=64, scale=0.0, window=0, sink=0, out=X, status=None, stream=None)
 
@@ -63,7 +63,7 @@ ATTN = [
 
 
 @pytest.mark.parametrize("kw,why", ATTN + [(dict(pos=None), b"null"), (dict(n=-1), b"sequences"),
-                                           (dict(n=65536), b"sequences")])
+                                           (dict(n=65536), b"sequences"), (dict(ws=X + 8, ws_bytes=64), b"workspace")])
 def test_decode_refusals(sfk, kw, why):
     assert call(sfk, "sfk_attn_decode_window", DECODE, **kw) == L.SFK_ERR_INVALID_ARGUMENT
     assert why in sfk.sfk_last_error()
