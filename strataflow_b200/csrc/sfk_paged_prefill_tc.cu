@@ -45,8 +45,8 @@ constexpr int TM = 128;       // rows per tile
 constexpr int TK = 128;       // keys per tile
 constexpr int TC_ROWS = 256;  // rows per CTA
 constexpr int TT = 384;       // threads: three warpgroups, 168 registers each at launch
-// Registers after the split: 2 x 128 x 216 + 128 x 72 = 384 x 168, what the launch holds
-constexpr int REG_SOFTMAX = 216, REG_OTHER = 72;
+// Registers after the split: 2 x 128 x 200 + 128 x 104 = 384 x 168, what the launch holds
+constexpr int REG_SOFTMAX = 200, REG_OTHER = 104;
 static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
 constexpr int PPT = TK / PG;  // pages per key tile
 
@@ -119,19 +119,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
       R16("f", v, 0)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld128(uint32_t addr, float (&v)[128]) {
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&v)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n"
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,"
-      "%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,"
-      "%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,"
-      "%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n"
+      "%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n"
       "tcgen05.wait::ld.sync.aligned;"
-      : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64), R32("=f", v, 96)
-      : "r"(addr), "r"(addr + 32), "r"(addr + 64), "r"(addr + 96)
+      : R32("=f", v, 0), R32("=f", v, 32)
+      : "r"(addr), "r"(addr + 32)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
@@ -360,16 +356,16 @@ __global__ void __launch_bounds__(TT, 1)
       for (int n = 0; n < nk; ++n) {
         if (!(ok = wait_warp(&c->s_full[w], n & 1, c, p.status))) break;
         fence_after();
-        float s[128];
-        tmem_ld128(ts, s);
         // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
         const int e0 = n * PPT;
         const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
                            (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
-        if (!inner) {
+        // keys 64 b .. 64 b + 63 of the tile that the row does not see become -inf
+        auto mask = [&](float (&s)[64], int b) {
 #pragma unroll
-          for (int g = 0; g < PPT; ++g) {
-            const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
+          for (int g = 0; g < 4; ++g) {
+            const int e = e0 + 4 * b + g;
+            const int jb = e < sp.n ? sp.page(e) * PG : 0x7fffff00;
             const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
 #pragma unroll
             for (int k = 0; k < PG; ++k) {
@@ -377,16 +373,22 @@ __global__ void __launch_bounds__(TT, 1)
               s[g * PG + k] = see ? s[g * PG + k] : -INFINITY;
             }
           }
-        }
-        float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+        };
+        // S is read twice, for the maximum and for P: 128 values held over would not leave registers for P
+        float mx = -INFINITY;
 #pragma unroll
-        for (int k = 4; k < 128; k += 4) {
-          mx0 = fmaxf(mx0, s[k]);
-          mx1 = fmaxf(mx1, s[k + 1]);
-          mx2 = fmaxf(mx2, s[k + 2]);
-          mx3 = fmaxf(mx3, s[k + 3]);
+        for (int b = 0; b < 2; ++b) {
+          float s[64];
+          tmem_ld64(ts + b * 64, s);
+          if (!inner) mask(s, b);
+          float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < 64; k += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
+          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
         }
-        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * scale;
+        mx *= scale;
         if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
           const float mn = fmaxf(mx, m);
           const float f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
@@ -405,31 +407,30 @@ __global__ void __launch_bounds__(TT, 1)
         }
         const float neg = BIAS - (m == -INFINITY ? 0.f : m);
         float l0 = 0.f, l1 = 0.f;
+        uint32_t lo[SPLIT ? 64 : 1];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {  // 64 keys: 32 columns of P
+        for (int b = 0; b < 2; ++b) {  // 64 keys: 32 columns of P, over S columns already read
+          float s[64];
+          tmem_ld64(ts + b * 64, s);
+          if (!inner) mask(s, b);
           uint32_t hi[32];
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
-            const float x = exp2_approx(fmaf(s[b * 64 + 2 * k], scale, neg));
-            const float y = exp2_approx(fmaf(s[b * 64 + 2 * k + 1], scale, neg));
+            const float x = exp2_approx(fmaf(s[2 * k], scale, neg));
+            const float y = exp2_approx(fmaf(s[2 * k + 1], scale, neg));
             l0 += x;
             l1 += y;
             hi[k] = pack2<BF16>(x, y);
             if constexpr (SPLIT) {
               const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-              s[b * 32 + k] = __uint_as_float(pack2<false>(x - f.x, y - f.y));
+              lo[b * 32 + k] = pack2<false>(x - f.x, y - f.y);
             }
           }
           tmem_st32(ts + b * 32, hi);
         }
         if constexpr (SPLIT) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            uint32_t lo[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) lo[k] = __float_as_uint(s[b * 32 + k]);
-            tmem_st32(ts + 64 + b * 32, lo);
-          }
+          for (int b = 0; b < 2; ++b) tmem_st32(ts + 64 + b * 32, reinterpret_cast<const uint32_t(&)[32]>(lo[b * 32]));
         }
         l += l0 + l1;
         tmem_st_wait();
