@@ -8,12 +8,12 @@
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: thread = TMEM lane = row.
 //                   Reads its S row, updates the running maximum, writes P over
 //                   S in TMEM as 16-bit A operands.
-//   warp 8          brings K and V tiles in, eight pages each, by tensor-map
+//   warps 8 and 10  bring K and V tiles in, eight pages each, by tensor-map
 //                   copies (128-byte swizzle) into a ring of tile slots.
 //   warp 9          one thread issues the products: P V of one row tile and the
 //                   next Q K^T of the same tile, then the other tile's, so the
 //                   tensor core works on one tile while the other is in softmax.
-//   warps 10, 11    fill the third warpgroup, which hands registers to the softmax.
+//   warp 11         fills the third warpgroup, which hands registers to the softmax.
 // S and O live in TMEM (2 x 128 and 2 x head_dim columns).  The products of one
 // thread run in order, so S(n + 1) of a row tile is complete only after its
 // P V(n): the softmax threads may touch O as soon as S(n + 1) has arrived.
@@ -45,10 +45,11 @@ constexpr int TM = 128;       // rows per tile
 constexpr int TK = 128;       // keys per tile
 constexpr int TC_ROWS = 256;  // rows per CTA
 constexpr int TT = 384;       // threads: three warpgroups, 168 registers each at launch
-// Registers after the split: 2 x 128 x 200 + 128 x 104 = 384 x 168, what the launch holds
-constexpr int REG_SOFTMAX = 200, REG_OTHER = 104;
+// Registers after the split: 2 x 128 x 208 + 128 x 88 = 384 x 168, what the launch holds
+constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
 static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
 constexpr int PPT = TK / PG;  // pages per key tile
+constexpr int POLY_OF_8 = 2;  // of 8 exponentials, how many go to the multiply-add unit
 
 template <int HD, bool SPLIT>
 struct Cfg {
@@ -65,31 +66,32 @@ struct Cfg {
 struct Ctl {
   uint64_t full[8], empty[8];
   uint64_t tail;     // the last V tile, before its rows past the end are zeroed
-  uint64_t q_ready[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_ready[2], s_full[2], p_full[2][2], o_full[2];  // p_full: [row tile][half of the keys]
   uint64_t drain;
   uint32_t tmem;
   int abort;
 };
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl* c, int* status) {
+// Bounded: false after about a second, or once another warp gave up.  Little code, for the loops that call it.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl* c) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 15) == 0) {
-      if (*(volatile int*)&c->abort) return false;
-      if (clock64() - t0 > (1ll << 31)) {  // about a second
-        *(volatile int*)&c->abort = 1;
-        report(status, ERR_TIMEOUT);
-        return false;
-      }
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > (1ll << 31) || *(volatile int*)&c->abort) {
+      *(volatile int*)&c->abort = 1;
+      return false;
     }
-  }
+  return true;
 }
-
 // the same for all lanes of a warp, which leave it together and with one answer
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Ctl* c, int* status) {
-  return __all_sync(0xffffffffu, wait(bar, parity, c, status));
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Ctl* c) {
+  return __all_sync(0xffffffffu, wait(bar, parity, c));
+}
+// one lane of the warp, always the same
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(on));
+  return on;
 }
 
 // ---- tcgen05 ------------------------------------------------------------------------
@@ -119,15 +121,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
       R16("f", v, 0)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&v)[64]) {
+__device__ __forceinline__ void tmem_ld128(uint32_t addr, float (&v)[128]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n"
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,"
-      "%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n"
+      "%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,"
+      "%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,"
+      "%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n"
       "tcgen05.wait::ld.sync.aligned;"
-      : R32("=f", v, 0), R32("=f", v, 32)
-      : "r"(addr), "r"(addr + 32)
+      : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64), R32("=f", v, 96)
+      : "r"(addr), "r"(addr + 32), "r"(addr + 64), "r"(addr + 96)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
@@ -141,29 +147,29 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Shared-memory matrix descriptor, 128-byte swizzle, version 1.  K-major: 8-row
+// groups 1024 bytes apart (the leading offset is not used).  MN-major: 64-element
+// column blocks `lbo` bytes apart, groups of 8 k-rows 1024 bytes apart.
+constexpr uint32_t DESC_HI = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | lbo >> 4 << 16; }
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
-// D += A B with A in shared memory / in TMEM, B in shared memory; f32 accumulator
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
-                   d),
-               "l"(a), "l"(b), "r"(idesc), "r"(acc)
-               : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D += A B with A in shared memory / in TMEM, B in shared memory; f32 accumulator.  a, b: low descriptor words.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
       : "memory");
 }
-// Shared-memory matrix descriptor, 128-byte swizzle, version 1.  K-major: 8-row
-// groups 1024 bytes apart (the leading offset is not used).  MN-major: 64-element
-// column blocks `lbo` bytes apart, groups of 8 k-rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 |
-         2ull << 61;
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
+      : "memory");
 }
 // instruction descriptor, kind::f16: D f32, A and B f16 (0) or bf16 (1), B K-major or MN-major
 __host__ __device__ constexpr uint32_t idesc_f16(int bf16, int n, int b_mn) {
@@ -176,6 +182,56 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// ---- two f32 at a time --------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float x) { return pair(x, x); }
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of a pair without the special-function unit, which has 4 lanes where the
+// multiply-add unit has 32: x = n + f with n the nearest whole number (the low
+// bits of x + 1.5 2^23), 2^f on [-1/2, 1/2] by a polynomial of least relative
+// error (Lawson's iteration), n added to the exponent.  Relative error 7.5e-5 at
+// degree 3, 2.7e-6 at degree 4: well below the rounding of P to bf16 (2^-8) and
+// f16 (2^-11).  x below -126 gives 2^-126.
+template <int DEG>
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
+  unpair(x2, x, y);
+  x2 = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t t = add2(x2, both(12582912.f));
+  const uint64_t f = fma2(add2(t, both(-12582912.f)), both(-1.f), x2);
+  uint64_t r;
+  if constexpr (DEG == 3) {
+    r = fma2(both(0.0551716685295105f), f, both(0.2426111251115799f));
+    r = fma2(r, f, both(0.6932609677314758f));
+    r = fma2(r, f, both(0.9999280571937561f));
+  } else {
+    r = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+    r = fma2(r, f, both(0.240247443318367f));
+    r = fma2(r, f, both(0.6931217908859253f));
+    r = fma2(r, f, both(0.9999992847442627f));
+  }
+  float a, b, u, v;
+  unpair(r, a, b);
+  unpair(t, u, v);
+  x = __int_as_float(__float_as_int(a) + (__float_as_int(u) << 23));
+  y = __int_as_float(__float_as_int(b) + (__float_as_int(v) << 23));
 }
 
 // ---- rows with a non-finite output ------------------------------------------------------
@@ -264,7 +320,8 @@ __global__ void __launch_bounds__(TT, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c->q_ready[i], TM);
       mbar_init(&c->s_full[i], 1);
-      mbar_init(&c->p_full[i], TM);
+      mbar_init(&c->p_full[i][0], 4);  // warps
+      mbar_init(&c->p_full[i][1], 4);
       mbar_init(&c->o_full[i], 1);
     }
     c->abort = 0;
@@ -353,41 +410,41 @@ __global__ void __launch_bounds__(TT, 1)
       constexpr float BIAS = SPLIT ? 15.f : 0.f;   // P = 2^BIAS at the maximum
       float m = -INFINITY, l = 0.f;  // m in scaled log2 units
       bool ok = true;
+      auto p_done = [&](int half) {  // this warp's rows of P are written
+        tmem_st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c->p_full[w][half]);
+      };
       for (int n = 0; n < nk; ++n) {
-        if (!(ok = wait_warp(&c->s_full[w], n & 1, c, p.status))) break;
+        if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
         fence_after();
         // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
         const int e0 = n * PPT;
         const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
                            (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
-        // keys 64 b .. 64 b + 63 of the tile that the row does not see become -inf
-        auto mask = [&](float (&s)[64], int b) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int e = e0 + 4 * b + g;
-            const int jb = e < sp.n ? sp.page(e) * PG : 0x7fffff00;
+        if (!inner) {
+          // what the row does not see becomes -inf, in place
+#pragma unroll 1
+          for (int g = 0; g < PPT; ++g) {
+            const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
             const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
+            float s[16];
+            tmem_ld16(ts + g * PG, s);
 #pragma unroll
-            for (int k = 0; k < PG; ++k) {
-              const bool see = k <= hi && (k > lo || k < sk);
-              s[g * PG + k] = see ? s[g * PG + k] : -INFINITY;
-            }
+            for (int k = 0; k < PG; ++k) s[k] = k <= hi && (k > lo || k < sk) ? s[k] : -INFINITY;
+            tmem_st16(ts + g * PG, s);
           }
-        };
-        // S is read twice, for the maximum and for P: 128 values held over would not leave registers for P
-        float mx = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          float s[64];
-          tmem_ld64(ts + b * 64, s);
-          if (!inner) mask(s, b);
-          float m4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int k = 4; k < 64; k += 4)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
-          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+          tmem_st_wait();
         }
+        float s[128];
+        tmem_ld128(ts, s);
+        float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int k = 4; k < 128; k += 4)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         mx *= scale;
         if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
           const float mn = fmaxf(mx, m);
@@ -406,40 +463,48 @@ __global__ void __launch_bounds__(TT, 1)
           }
         }
         const float neg = BIAS - (m == -INFINITY ? 0.f : m);
-        float l0 = 0.f, l1 = 0.f;
+        const uint64_t scale2 = both(scale), neg2 = both(neg);
+        uint64_t sum2 = 0;
         uint32_t lo[SPLIT ? 64 : 1];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {  // 64 keys: 32 columns of P, over S columns already read
-          float s[64];
-          tmem_ld64(ts + b * 64, s);
-          if (!inner) mask(s, b);
-          uint32_t hi[32];
+        for (int b = 0; b < 4; ++b) {  // 32 keys: 16 columns of P, over S columns already read
+          uint32_t hi[16];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float x = exp2_approx(fmaf(s[2 * k], scale, neg));
-            const float y = exp2_approx(fmaf(s[2 * k + 1], scale, neg));
-            l0 += x;
-            l1 += y;
+          for (int k = 0; k < 16; ++k) {
+            const uint64_t x2 = fma2(pair(s[b * 32 + 2 * k], s[b * 32 + 2 * k + 1]), scale2, neg2);
+            float x, y;
+            if (!SPLIT && (k * 3) % 8 < POLY_OF_8) {
+              exp2_poly<BF16 ? 3 : 4>(x2, x, y);
+            } else {
+              unpair(x2, x, y);
+              x = exp2_approx(x);
+              y = exp2_approx(y);
+            }
+            sum2 = add2(sum2, pair(x, y));
             hi[k] = pack2<BF16>(x, y);
             if constexpr (SPLIT) {
               const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-              lo[b * 32 + k] = pack2<false>(x - f.x, y - f.y);
+              lo[b * 16 + k] = pack2<false>(x - f.x, y - f.y);
             }
           }
-          tmem_st32(ts + b * 32, hi);
+          tmem_st16(ts + b * 16, reinterpret_cast<const float(&)[16]>(hi));
+          if (!SPLIT && b == 1) {  // the product of these keys may begin
+            p_done(0);
+          }
         }
         if constexpr (SPLIT) {
 #pragma unroll
           for (int b = 0; b < 2; ++b) tmem_st32(ts + 64 + b * 32, reinterpret_cast<const uint32_t(&)[32]>(lo[b * 32]));
         }
+        float l0, l1;
+        unpair(sum2, l0, l1);
         l += l0 + l1;
-        tmem_st_wait();
-        fence_before();
-        mbar_arrive(&c->p_full[w]);
+        if (SPLIT) p_done(0);
+        p_done(1);
       }
       // ---- out = O / l ----
       if (nk > 0 && ok) {
-        ok = wait_warp(&c->o_full[w], 0, c, p.status);
+        ok = wait_warp(&c->o_full[w], 0, c);
         fence_after();
       }
       if (ok) {
@@ -477,104 +542,123 @@ __global__ void __launch_bounds__(TT, 1)
     }
   } else {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
-  if (warp == 8) {
-    // ---- K and V tiles ----
-    const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
+  if (warp == 8 || warp == 10) {
+    // ---- K tiles (warp 8) and V tiles (warp 10) ----
+    const int v = warp == 10;
+    const CUtensorMap* map = v ? &vmap : &kmap;
+    const int past_end = p.n_pages * p.n_head_kv * PG;  // a row outside the map: zeros
     const int* table = p.page_table + (int64_t)t.seq * p.max_pages;
     const int kv_end = t.past + t.n_q;  // keys of the sequence
-    bool ok = true;
-    for (int n = 0; n < nk && ok; ++n) {
-      // lane i < 8: row of page i in the map; outside it (zeros) where there is none
-      int y = (int)rows;
-      if (lane < PPT && n * PPT + lane < sp.n) {
-        const int id = table[sp.page(n * PPT + lane)];
+    // lane i: row in the map of page entry e + i, for the 32 entries (four tiles) from e
+    auto rows_from = [&](int e) {
+      int y = past_end;
+      if (e + lane < sp.n) {
+        const int id = table[sp.page(e + lane)];
         if (id >= 0 && id < p.n_pages) y = (id * p.n_head_kv + hk) * PG;
         else report(p.status, ERR_BAD_PAGE);
       }
-      // rows of the last page past the sequence's end
-      const int n_tail = n == nk - 1 ? (sp.page(sp.n - 1) + 1) * PG - kv_end : 0;
-      for (int v = 0; v < 2 && ok; ++v) {
-        const int i = 2 * n + v, slot = i % C::STAGES;
-        if (i >= C::STAGES && !(ok = wait_warp(&c->empty[slot], (uint32_t)(i / C::STAGES - 1) & 1, c, p.status))) break;
-        const bool fix = v && n_tail > 0;
-        uint64_t* bar = fix ? &c->tail : &c->full[slot];
-        if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
-        __syncwarp();
-        const uint32_t dst = smem_u32(ring + slot * C::TILE);
-        const int yy = __shfl_sync(0xffffffffu, y, lane % PPT);
-        if (lane < PPT * C::HALVES)
-          tma_page(dst + (lane / PPT) * (TK * 128) + (lane % PPT) * (PG * 128), v ? &vmap : &kmap, yy, bar, lane / PPT);
-        __syncwarp();
-        if (fix) {
-          ok = wait_warp(&c->tail, 0, c, p.status);
-          const int key0 = (sp.n - 1 - n * PPT) * PG + PG - n_tail;
-          for (int x = lane; x < n_tail * 8 * C::HALVES; x += 32) {
-            const int key = key0 + x / 8 % n_tail, half = x / 8 / n_tail;
-            *reinterpret_cast<uint4*>(ring + slot * C::TILE + half * (TK * 128) + key * 128 + x % 8 * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&c->full[slot]);
-        }
+      return y;
+    };
+    int ahead = rows_from(0), y = past_end;
+    bool ok = true;
+    int slot = v % C::STAGES;
+    uint32_t use = v / C::STAGES;  // how often the slot was filled before
+    for (int n = 0; n < nk && ok; ++n) {
+      if (n % 4 == 0) {
+        y = ahead;
+        ahead = rows_from((n + 4) * PPT);
       }
+      // rows of the last page past the sequence's end
+      const int n_tail = v && n == nk - 1 ? (sp.page(sp.n - 1) + 1) * PG - kv_end : 0;
+      if (use > 0 && !(ok = wait_warp(&c->empty[slot], (use - 1) & 1, c))) break;
+      uint64_t* bar = n_tail > 0 ? &c->tail : &c->full[slot];
+      if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+      __syncwarp();
+      const uint32_t dst = smem_u32(ring + slot * C::TILE);
+      const int yy = __shfl_sync(0xffffffffu, y, n % 4 * PPT + lane % PPT);
+      if (lane < PPT * C::HALVES)
+        tma_page(dst + (lane / PPT) * (TK * 128) + (lane % PPT) * (PG * 128), map, yy, bar, lane / PPT);
+      __syncwarp();
+      if (n_tail > 0) {
+        ok = wait_warp(&c->tail, 0, c);
+        const int key0 = (sp.n - 1 - n * PPT) * PG + PG - n_tail;
+        for (int x = lane; x < n_tail * 8 * C::HALVES; x += 32) {
+          const int key = key0 + x / 8 % n_tail, half = x / 8 / n_tail;
+          *reinterpret_cast<uint4*>(ring + slot * C::TILE + half * (TK * 128) + key * 128 + x % 8 * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c->full[slot]);
+      }
+      if ((slot += 2) >= C::STAGES) slot -= C::STAGES, ++use;
     }
-  } else if (warp == 9 && lane == 0) {
+  } else if (warp == 9) {
     // ---- products ----
     constexpr uint32_t QK = idesc_f16(BF16, TK, 0), PV = idesc_f16(BF16, HDP, 1);
-    const uint32_t q_addr = smem_u32(qs), ring_addr = smem_u32(ring);
-    auto qk = [&](int w, int n) {
-      const uint32_t k_addr = ring_addr + (2 * n % C::STAGES) * C::TILE;
+    const uint32_t q_lo = desc_lo(smem_u32(qs), 16), k_lo = desc_lo(smem_u32(ring), 16);
+    const uint32_t v_lo = desc_lo(smem_u32(ring), TK * 128);
+    auto qk = [&](int w, int slot) {
+      const uint32_t a = q_lo + w * (NS * C::TILE >> 4), b = k_lo + slot * (C::TILE >> 4), d = tmem + w * 128;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
         for (int k = 0; k < HDP / 16; ++k) {
-          const uint32_t off = (k / 4) * (TM * 128) + (k % 4) * 32;
-          mma_ss(tmem + w * 128, desc128(q_addr + (w * NS + s) * C::TILE + off, 16), desc128(k_addr + off, 16), QK, s + k > 0);
+          const uint32_t off = ((k / 4) * (TM * 128) + (k % 4) * 32) >> 4;
+          mma_ss(d, a + (s * C::TILE >> 4) + off, b + off, QK, s + k > 0);
         }
-      commit(&c->s_full[w]);
     };
-    auto pv = [&](int w, int n) {
-      const uint32_t v_addr = ring_addr + ((2 * n + 1) % C::STAGES) * C::TILE;
+    auto pv = [&](int w, int slot, int half, uint32_t acc) {
+      const uint32_t a = tmem + w * 128 + half * (TK / 4), b = v_lo + ((slot * C::TILE + half * (TK / 2) * 128) >> 4);
+      const uint32_t d = tmem + 256 + w * HDP;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int k = 0; k < TK / 16; ++k)
-          mma_ts(tmem + 256 + w * HDP, tmem + w * 128 + s * 64 + k * 8, desc128(v_addr + k * 2048, TK * 128), PV,
-                 n > 0 || s + k > 0);
+        for (int k = 0; k < TK / 32; ++k) mma_ts(d, a + s * 64 + k * 8, b + (k * 2048 >> 4), PV, s + k > 0 ? 1 : acc);
     };
-    bool ok = nk > 0;
-    for (int w = 0; w < n_tiles && ok; ++w) {
-      ok = wait(&c->q_ready[w], 0, c, p.status);
-      if (ok && w == 0) ok = wait(&c->full[0], 0, c, p.status);
-      if (!ok) break;
-      fence_after();
-      qk(w, 0);
-    }
-    if (ok) commit(&c->empty[0]);
-    for (int n = 0; n < nk && ok; ++n) {
-      const int iv = 2 * n + 1, ik = 2 * n + 2;
-      if (!(ok = wait(&c->full[iv % C::STAGES], (uint32_t)(iv / C::STAGES) & 1, c, p.status))) break;
-      for (int w = 0; w < n_tiles; ++w) {
-        if (!(ok = wait(&c->p_full[w], n & 1, c, p.status))) break;
+    if (elect_one()) {  // one thread for the whole loop: a vote or a warp barrier at each wait costs more than the wait
+      bool ok = nk > 0;
+      if (ok) ok = wait(&c->full[0], 0, c);
+      for (int w = 0; w < n_tiles && ok; ++w) {
+        if (!(ok = wait(&c->q_ready[w], 0, c))) break;
         fence_after();
-        pv(w, n);
-        if (w == n_tiles - 1) commit(&c->empty[iv % C::STAGES]);
-        if (n + 1 < nk) {
-          if (w == 0 && !(ok = wait(&c->full[ik % C::STAGES], (uint32_t)(ik / C::STAGES) & 1, c, p.status))) break;
-          qk(w, n + 1);
-          if (w == n_tiles - 1) commit(&c->empty[ik % C::STAGES]);
-        } else {
-          commit(&c->o_full[w]);
+        qk(w, 0);
+        commit(&c->s_full[w]);
+        if (w == n_tiles - 1) commit(&c->empty[0]);
+      }
+      int sv = 1 % C::STAGES, sk = 2 % C::STAGES;   // slots of V(n), K(n + 1) and their phases
+      uint32_t fv = 1 / C::STAGES, fk = 2 / C::STAGES;
+      for (int n = 0; n < nk && ok; ++n) {
+        const bool more = n + 1 < nk;
+        if (!(ok = wait(&c->full[sv], fv & 1, c))) break;
+        if (more && !(ok = wait(&c->full[sk], fk & 1, c))) break;
+#pragma unroll 1
+        for (int w = 0; w < n_tiles; ++w) {
+          if (!(ok = wait(&c->p_full[w][0], n & 1, c))) break;
+          fence_after();
+          pv(w, sv, 0, n > 0);
+          if (!(ok = wait(&c->p_full[w][1], n & 1, c))) break;
+          fence_after();
+          pv(w, sv, 1, 1);
+          if (more) qk(w, sk);
+          commit(more ? &c->s_full[w] : &c->o_full[w]);
+          if (w == n_tiles - 1) {
+            commit(&c->empty[sv]);
+            if (more) commit(&c->empty[sk]);
+          }
         }
+        if ((sv += 2) >= C::STAGES) sv -= C::STAGES, ++fv;
+        if ((sk += 2) >= C::STAGES) sk -= C::STAGES, ++fk;
       }
     }
+    __syncwarp();
   }
   }
   __syncwarp();
   fence_before();
   __syncthreads();
   if (*(volatile int*)&c->abort) {
+    if (tid == 0) report(p.status, ERR_TIMEOUT);
     // a wait ran out: the products and copies still under way end before the memory goes
     if (warp == 9 && lane == 0) {
       commit(&c->drain);
