@@ -350,56 +350,74 @@ __global__ void __launch_bounds__(TT, 1)
       const int t_lo = t.past + (t.row0 + w * TM) / G;
       const int t_hi = t.past + (t.row0 + min(n_rows, w * TM + TM) - 1) / G;
       float scale = p.scale_log2;
-      {
-        // q into shared memory, swizzled: 16-byte chunk i of the row's 128-byte block at i ^ (row % 8)
-        const int lr = row % TM;
-        uint8_t* q0 = qs + w * NS * C::TILE + lr * 128;
-        const int64_t at = (int64_t)(t.q0 + tok) * p.q_stride + (int64_t)h * HD;
-        float up = 1.f;
-        if (SPLIT && live) {
-          float mx = 0.f;
-          for (int d = 0; d < HD; d += 8) {
-            Raw8<float> raw;
-            float x[8];
-            load8(raw, static_cast<const float*>(p.q) + at + d, p.q_vec);
-            unpack8(raw, x);
+      const int wrow = w * TM + (warp % 4) * 32;  // first row of the warp
+      // A row of q by HD / 8 lanes, 16 bytes of a 16-bit type each, two or more rows at a time (thread by row
+      // instead, the loads of a warp go to 32 rows: measured 10k cycles for the tile, and this is before the
+      // first product).  Into shared memory swizzled: 16-byte chunk i of the row's 128-byte block at i ^ (row % 8).
+      constexpr int LR = HD / 8, RI = 32 / LR;  // lanes per row, rows per step
+      const int64_t my_q = live ? (int64_t)(t.q0 + tok) * p.q_stride + (int64_t)h * HD : -1;
+      if (nk > 0) {
+        const int ch = lane % LR;
+        auto slot = [&](int lr, int c) {  // row of the tile, chunk of the row
+          return qs + w * NS * C::TILE + lr * 128 + c / 8 * (TM * 128) + ((c % 8) ^ (lr & 7)) * 16;
+        };
+        if constexpr (SPLIT) {
+#pragma unroll 1
+          for (int i0 = 0; i0 < LR; i0 += (LR < 8 ? LR : 8)) {
+            constexpr int B = LR < 8 ? LR : 8;
+            Raw8<float> raw[B];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+            for (int i = 0; i < B; ++i) {
+              const int64_t at = __shfl_sync(0xffffffffu, my_q, (i0 + i) * RI + lane / LR);
+              raw[i].w[0] = raw[i].w[1] = make_uint4(0, 0, 0, 0);
+              if (at >= 0) load8(raw[i], static_cast<const float*>(p.q) + at + ch * 8, p.q_vec);
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+              const int rr = (i0 + i) * RI + lane / LR;  // row of the warp
+              float x[8], mx = 0.f;
+              unpack8(raw[i], x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+              for (int d = 1; d < LR; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              // the row's largest |q| to [1, 2): a power of two, exact, undone in the row's scale
+              int e = (int)(__float_as_uint(mx) >> 23) - 127;
+              e = mx > 0.f && e < 128 ? min(max(e, -126), 126) : 0;
+              const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+              const int er = __shfl_sync(0xffffffffu, e, lane % RI * LR);
+              if (lane / RI == i0 + i) scale = p.scale_log2 * __uint_as_float((uint32_t)(er + 127) << 23);
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float u = x[2 * k] * up, v = x[2 * k + 1] * up;
+                hi[k] = pack2<false>(u, v);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                lo[k] = pack2<false>(u - f.x, v - f.y);
+              }
+              uint8_t* dst = slot(wrow % TM + rr, ch);
+              *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4*>(dst + C::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
           }
-          // largest |q| to [1, 2): exact, and undone in the scale
-          int e = (int)(__float_as_uint(mx) >> 23) - 127;
-          if (mx > 0.f && e < 128) {
-            e = max(e, -126);
-            up = exp2f((float)-e);  // a power of two: exact
-            scale *= exp2f((float)e);
+        } else {
+          Raw8<KV> raw[LR];
+#pragma unroll
+          for (int i = 0; i < LR; ++i) {
+            const int64_t at = __shfl_sync(0xffffffffu, my_q, i * RI + lane / LR);
+            raw[i].w[0] = make_uint4(0, 0, 0, 0);
+            if (at >= 0) load8(raw[i], static_cast<const KV*>(p.q) + at + ch * 8, p.q_vec);
           }
+#pragma unroll
+          for (int i = 0; i < LR; ++i)
+            *reinterpret_cast<uint4*>(slot(wrow % TM + i * RI + lane / LR, ch)) = raw[i].w[0];
         }
-#pragma unroll 2
-        for (int d = 0; d < HDP; d += 8) {
-          uint8_t* dst = q0 + (d / 64) * (TM * 128) + ((((d % 64) / 8) ^ (lr & 7)) * 16);
-          if constexpr (SPLIT) {
-            float x[8] = {};
-            if (live && d < HD) {
-              Raw8<float> raw;
-              load8(raw, static_cast<const float*>(p.q) + at + d, p.q_vec);
-              unpack8(raw, x);
-            }
-            uint32_t hi[4], lo[4];
+        if constexpr (HDP > HD) {  // dims past the head
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = x[2 * e] * up, b = x[2 * e + 1] * up;
-              hi[e] = pack2<false>(a, b);
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-              lo[e] = pack2<false>(a - f.x, b - f.y);
-            }
-            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(dst + C::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          } else {
-            Raw8<KV> raw;
-            raw.w[0] = make_uint4(0, 0, 0, 0);
-            if (live && d < HD) load8(raw, static_cast<const KV*>(p.q) + at + d, p.q_vec);
-            *reinterpret_cast<uint4*>(dst) = raw.w[0];
-          }
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = HD / 8; k < HDP / 8; ++k)
+              *reinterpret_cast<uint4*>(slot(wrow % TM + lane, k) + s * C::TILE) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         mbar_arrive(&c->q_ready[w]);
@@ -508,25 +526,50 @@ __global__ void __launch_bounds__(TT, 1)
         fence_after();
       }
       if (ok) {
+        // Through shared memory (the tile's q, whose products are done), so that a warp writes whole rows: 16-byte
+        // chunk i of a row at i ^ (row % 8).
+        constexpr int ES = SPLIT ? 4 : 2, CH = HD * ES / 16;  // bytes of an output element, chunks of a row
+        constexpr int X = CH < 8 ? CH - 1 : 7;
+        uint8_t* rows = qs + w * NS * C::TILE + wrow % TM * (HD * ES);
         const float inv = 1.0f / l;
         bool finite = true;
 #pragma unroll 1
         for (int d = 0; d < HD; d += 32) {
           float o[32];
-          __syncwarp();
           if (nk > 0) tmem_ld32(to + d, o);
-          if (live) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              finite = finite && fabsf(o[k]) < INFINITY;
-              o[k] = pos >= 0 ? o[k] * inv : 0.f;
-            }
-            const int64_t at = ((int64_t)(t.q0 + tok) * p.n_head + h) * HD + d;
+          for (int k = 0; k < 32; ++k) {
+            finite = finite && fabsf(o[k]) < INFINITY;
+            o[k] = pos >= 0 ? o[k] * inv : 0.f;
+          }
+          uint8_t* mine = rows + lane * (HD * ES);
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              const float(&x)[8] = *reinterpret_cast<const float(*)[8]>(&o[k]);
-              if (SPLIT) store8(static_cast<float*>(p.out) + at + k, x, p.out_vec);
-              else store8(static_cast<KV*>(p.out) + at + k, x, p.out_vec);
+          for (int k = 0; k < 32; k += 16 / ES) {
+            uint4 v;
+            if constexpr (SPLIT)
+              v = make_uint4(__float_as_uint(o[k]), __float_as_uint(o[k + 1]), __float_as_uint(o[k + 2]), __float_as_uint(o[k + 3]));
+            else
+              v = make_uint4(pack2<BF16>(o[k], o[k + 1]), pack2<BF16>(o[k + 2], o[k + 3]), pack2<BF16>(o[k + 4], o[k + 5]),
+                             pack2<BF16>(o[k + 6], o[k + 7]));
+            *reinterpret_cast<uint4*>(mine + ((((d + k) * ES / 16) ^ (lane & X)) * 16)) = v;
+          }
+        }
+        __syncwarp();
+        const int64_t my_out = live ? ((int64_t)(t.q0 + tok) * p.n_head + h) * HD : -1;
+        constexpr int RO = 32 / CH;  // rows per step
+#pragma unroll 4
+        for (int i = 0; i < CH; ++i) {
+          const int rr = i * RO + lane / CH, ch = lane % CH;
+          const int64_t at = __shfl_sync(0xffffffffu, my_out, rr);
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + rr * (HD * ES) + ((ch ^ (rr & X)) * 16));
+          if (at >= 0) {
+            uint8_t* dst = static_cast<uint8_t*>(p.out) + (at * ES + ch * 16);
+            if (p.out_vec) {
+              *reinterpret_cast<uint4*>(dst) = v;
+            } else {  // rows off 16-byte boundaries
+              const uint16_t* e = reinterpret_cast<const uint16_t*>(&v);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = e[k];
             }
           }
         }
