@@ -4,19 +4,21 @@
 //   S = Q K^T;  P = 2^(scale S - m);  O = sum over key tiles of P V;  out = O / sum P
 //
 // A CTA takes two tiles of 128 rows (rows: tokens x the query heads of one kv
-// head) and walks the pages its rows see in tiles of 128 keys:
+// head) and walks the pages its rows see in tiles of TK keys:
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: thread = TMEM lane = row.
-//                   Reads its S row, updates the running maximum, writes P over
-//                   S in TMEM as 16-bit A operands.
-//   warps 8 and 10  bring K and V tiles in, eight pages each, by tensor-map
-//                   copies (128-byte swizzle) into a ring of tile slots.
-//   warp 9          one thread issues the products: P V of one row tile and the
-//                   next Q K^T of the same tile, then the other tile's, so the
-//                   tensor core works on one tile while the other is in softmax.
-//   warp 11         fills the third warpgroup, which hands registers to the softmax.
-// S and O live in TMEM (2 x 128 and 2 x head_dim columns).  The products of one
-// thread run in order, so S(n + 1) of a row tile is complete only after its
-// P V(n): the softmax threads may touch O as soon as S(n + 1) has arrived.
+//                   Reads its S row into registers, updates the running maximum,
+//                   writes P to TMEM as 16-bit A operands.
+//   warps 8 and 10  bring K and V tiles in, page by page, by tensor-map copies
+//                   (128-byte swizzle), into a ring of tiles each.
+//   warps 9 and 11  one thread each issues Q K^T and P V of both row tiles.
+// S, P and O of both row tiles live in TMEM side by side: S(n + 1) is computed as
+// soon as S(n) is in registers, under the exponentials of S(n), so a softmax warp
+// goes from tile to tile without waiting for the tensor core.  That sets TK: 80 keys
+// at head width 128 (S 2 x 80, P 2 x 40, O 2 x 128 of 512 columns), 128 at 64.
+// (P over S with 128 keys, the products of a tile in one chain with its softmax, took
+// 892 us for 2048 tokens at 30000 keys, 32 heads of 128.)
+// One thread issues in about 30 cycles a product and 100 a wait: Q K^T and P V
+// by one thread were what the kernel waited for.
 //
 // The running maximum m is only raised when a row outgrows it by 2^8: O is
 // rescaled then, by the row's own thread.  P then reaches 2^8, far inside both
@@ -42,31 +44,40 @@ namespace sfk {
 namespace {
 
 constexpr int TM = 128;       // rows per tile
-constexpr int TK = 128;       // keys per tile
 constexpr int TC_ROWS = 256;  // rows per CTA
 constexpr int TT = 384;       // threads: three warpgroups, 168 registers each at launch
-// Registers after the split: 2 x 128 x 208 + 128 x 88 = 384 x 168, what the launch holds
-constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
-static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
-constexpr int PPT = TK / PG;  // pages per key tile
 constexpr int POLY_OF_8 = 2;  // of 8 exponentials, how many go to the multiply-add unit
 
 template <int HD, bool SPLIT>
 struct Cfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;  // head width in shared memory (the copy fills with zeros)
   static constexpr int HALVES = HDP / 64;        // 128-byte column blocks
-  static constexpr int TILE = TK * HDP * 2;      // bytes of a K, V or Q tile
   static constexpr int NS = SPLIT ? 2 : 1;       // terms of q and P
-  static constexpr int QB = 2 * NS * TILE;
-  static constexpr int FIT = (224 * 1024 - QB) / TILE;
-  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
-  static constexpr int SMEM = 1024 + QB + STAGES * TILE + 512;
+  // Keys per tile: S (TK columns), P (TK / 2 a term) and O (HDP) of two row tiles share the 512 columns of TMEM
+  static constexpr int TK = HDP == 64 ? (SPLIT ? 96 : 128) : (SPLIT ? 64 : 80);
+  static constexpr int PPT = TK / PG;            // pages per key tile
+  static constexpr int TILE = TK * HDP * 2;      // bytes of a K or V tile
+  static constexpr int QTILE = TM * HDP * 2;     // bytes of a q term of a row tile
+  static constexpr int QB = 2 * NS * QTILE;
+  static constexpr int FIT = (224 * 1024 - QB) / (2 * TILE);
+  static constexpr int STAGES = FIT > 4 ? 4 : FIT;  // K tiles, and V tiles, under way
+  static constexpr int SMEM = 1024 + QB + 2 * STAGES * TILE + 512;
+  static constexpr int FIRST = (PPT + 1) / 2 * PG;  // keys of the first part of P
+  // Registers after the split: 384 x 168 is what the launch holds.  A softmax thread holds a row of S.
+  static constexpr int REG_SOFTMAX = TK == 128 ? 208 : 184, REG_OTHER = TK == 128 ? 88 : 136;
+  static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
+  // TMEM columns
+  static constexpr int P0 = 2 * TK, PCOLS = TK / 2 * NS, O0 = 512 - 2 * HDP;
+  static_assert(P0 + 2 * PCOLS <= O0 && STAGES >= 2 && TK % PG == 0, "tile sizes");
 };
 
 struct Ctl {
-  uint64_t full[8], empty[8];
-  uint64_t tail;     // the last V tile, before its rows past the end are zeroed
-  uint64_t q_ready[2], s_full[2], p_full[2][2], o_full[2];  // p_full: [row tile][half of the keys]
+  uint64_t full[2][4], empty[2][4];  // [K, V][stage]
+  uint64_t tail;                     // the last V tile, before its rows past the end are zeroed
+  uint64_t q_ready[2];
+  uint64_t s_full[2], s_free[2];     // S of a row tile is complete / is in registers
+  uint64_t p_full[2][2];             // [row tile][part of the keys]: P is written
+  uint64_t pv_done[2];               // O is complete and P is free
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -121,27 +132,61 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
       R16("f", v, 0)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld128(uint32_t addr, float (&v)[128]) {
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,"
-      "%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,"
-      "%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,"
-      "%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R32("=f", v, 0), R32("=f", v, 32)
+      : "r"(addr), "r"(addr + 32)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[80]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%80];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%81];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79},"
+      " [%82];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R32("=f", v, 0), R32("=f", v, 32), R16("=f", v, 64)
+      : "r"(addr), "r"(addr + 32), "r"(addr + 64)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[96]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%96];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%97];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%98];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64)
+      : "r"(addr), "r"(addr + 32), "r"(addr + 64)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,"
+      "%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64), R32("=f", v, 96)
       : "r"(addr), "r"(addr + 32), "r"(addr + 64), "r"(addr + 96)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      R32("r", v, 0)
-      : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), R8("r", v, 0)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -291,12 +336,12 @@ __global__ void __launch_bounds__(TT, 1)
                       const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<HD, SPLIT>;
   constexpr bool BF16 = std::is_same<KV, __nv_bfloat16>::value;
-  constexpr int HDP = C::HDP, NS = C::NS;
+  constexpr int HDP = C::HDP, NS = C::NS, TK = C::TK, PPT = C::PPT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = base;                   // [tile][term][half][128 rows][128 B]
-  uint8_t* ring = base + C::QB;         // [stage][half][128 keys][128 B]
-  Ctl* c = reinterpret_cast<Ctl*>(base + C::QB + C::STAGES * C::TILE);
+  uint8_t* ring = base + C::QB;         // [K, V][stage][half][TK keys][128 B]
+  Ctl* c = reinterpret_cast<Ctl*>(base + C::QB + 2 * C::STAGES * C::TILE);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int G = p.n_head / p.n_head_kv, hk = blockIdx.x % p.n_head_kv;
 
@@ -311,18 +356,20 @@ __global__ void __launch_bounds__(TT, 1)
   const int nk = (sp.n + PPT - 1) / PPT;
 
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) {
-      mbar_init(&c->full[i], 1);
-      mbar_init(&c->empty[i], 1);
-    }
+    for (int v = 0; v < 2; ++v)
+      for (int i = 0; i < C::STAGES; ++i) {
+        mbar_init(&c->full[v][i], 1);
+        mbar_init(&c->empty[v][i], 1);
+      }
     mbar_init(&c->tail, 1);
-    mbar_init(&c->drain, 1);
+    mbar_init(&c->drain, 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c->q_ready[i], TM);
       mbar_init(&c->s_full[i], 1);
-      mbar_init(&c->p_full[i][0], 4);  // warps
+      mbar_init(&c->s_free[i], 4);  // warps
+      mbar_init(&c->p_full[i][0], 4);
       mbar_init(&c->p_full[i][1], 4);
-      mbar_init(&c->o_full[i], 1);
+      mbar_init(&c->pv_done[i], 1);
     }
     c->abort = 0;
     fence_mbar_init();
@@ -335,10 +382,10 @@ __global__ void __launch_bounds__(TT, 1)
   }
   __syncthreads();
   fence_after();
-  const uint32_t tmem = c->tmem;  // S tiles at 0 and 128, O tiles at 256 and 256 + HDP
+  const uint32_t tmem = c->tmem;
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFTMAX));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFTMAX));
     // ---- softmax: thread = row ----
     const int w = warp / 4;  // row tile
     if (w < n_tiles) {
@@ -359,7 +406,7 @@ __global__ void __launch_bounds__(TT, 1)
       if (nk > 0) {
         const int ch = lane % LR;
         auto slot = [&](int lr, int c) {  // row of the tile, chunk of the row
-          return qs + w * NS * C::TILE + lr * 128 + c / 8 * (TM * 128) + ((c % 8) ^ (lr & 7)) * 16;
+          return qs + w * NS * C::QTILE + lr * 128 + c / 8 * (TM * 128) + ((c % 8) ^ (lr & 7)) * 16;
         };
         if constexpr (SPLIT) {
 #pragma unroll 1
@@ -397,7 +444,7 @@ __global__ void __launch_bounds__(TT, 1)
               }
               uint8_t* dst = slot(wrow % TM + rr, ch);
               *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              *reinterpret_cast<uint4*>(dst + C::TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              *reinterpret_cast<uint4*>(dst + C::QTILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
           }
         } else {
@@ -417,22 +464,21 @@ __global__ void __launch_bounds__(TT, 1)
           for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int k = HD / 8; k < HDP / 8; ++k)
-              *reinterpret_cast<uint4*>(slot(wrow % TM + lane, k) + s * C::TILE) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(slot(wrow % TM + lane, k) + s * C::QTILE) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         mbar_arrive(&c->q_ready[w]);
       }
       const uint32_t lanes = (uint32_t)(warp % 4) * 32 << 16;
-      const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + 256 + w * HDP;
+      const uint32_t ts = tmem + lanes + w * TK, tp = tmem + lanes + C::P0 + w * C::PCOLS, to = tmem + lanes + C::O0 + w * HDP;
       constexpr float RAISE = SPLIT ? 0.f : 8.f;   // log2 by which a row may outgrow m
       constexpr float BIAS = SPLIT ? 15.f : 0.f;   // P = 2^BIAS at the maximum
       float m = -INFINITY, l = 0.f;  // m in scaled log2 units
       bool ok = true;
-      auto p_done = [&](int half) {  // this warp's rows of P are written
-        tmem_st_wait();
+      auto done = [&](uint64_t* bar) {  // what this warp's lanes did in TMEM so far
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&c->p_full[w][half]);
+        if (lane == 0) mbar_arrive(bar);
       };
       for (int n = 0; n < nk; ++n) {
         if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
@@ -455,21 +501,27 @@ __global__ void __launch_bounds__(TT, 1)
           }
           tmem_st_wait();
         }
-        float s[128];
-        tmem_ld128(ts, s);
+        float s[TK];
+        tmem_ld(ts, s);
+        if (n + 1 < nk) done(&c->s_free[w]);  // the next Q K^T may begin
         float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int k = 4; k < 128; k += 4)
+        for (int k = 4; k < TK; k += 4)
 #pragma unroll
           for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        // O is complete and P may be written again (mostly long since)
+        if (n > 0) {
+          if (!(ok = wait_warp(&c->pv_done[w], (n - 1) & 1, c))) break;
+          fence_after();
+        }
         mx *= scale;
         if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
           const float mn = fmaxf(mx, m);
           const float f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
           m = mn;
           l *= f;
-          if (n > 0) {  // O is complete: S(n) came after P V(n - 1)
+          if (n > 0) {
 #pragma unroll 1
             for (int d = 0; d < HDP; d += 16) {
               float o[16];
@@ -483,13 +535,12 @@ __global__ void __launch_bounds__(TT, 1)
         const float neg = BIAS - (m == -INFINITY ? 0.f : m);
         const uint64_t scale2 = both(scale), neg2 = both(neg);
         uint64_t sum2 = 0;
-        uint32_t lo[SPLIT ? 64 : 1];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {  // 32 keys: 16 columns of P, over S columns already read
-          uint32_t hi[16];
+        for (int b = 0; b < PPT; ++b) {  // 16 keys: 8 columns of P
+          uint32_t hi[8], lo[8];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const uint64_t x2 = fma2(pair(s[b * 32 + 2 * k], s[b * 32 + 2 * k + 1]), scale2, neg2);
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, neg2);
             float x, y;
             if (!SPLIT && (k * 3) % 8 < POLY_OF_8) {
               exp2_poly<BF16 ? 3 : 4>(x2, x, y);
@@ -502,27 +553,25 @@ __global__ void __launch_bounds__(TT, 1)
             hi[k] = pack2<BF16>(x, y);
             if constexpr (SPLIT) {
               const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-              lo[b * 16 + k] = pack2<false>(x - f.x, y - f.y);
+              lo[k] = pack2<false>(x - f.x, y - f.y);
             }
           }
-          tmem_st16(ts + b * 16, reinterpret_cast<const float(&)[16]>(hi));
-          if (!SPLIT && b == 1) {  // the product of these keys may begin
-            p_done(0);
+          tmem_st8(tp + b * 8, hi);
+          if constexpr (SPLIT) tmem_st8(tp + TK / 2 + b * 8, lo);
+          if ((b + 1) * PG == C::FIRST) {  // the product of these keys may begin
+            tmem_st_wait();
+            done(&c->p_full[w][0]);
           }
-        }
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b) tmem_st32(ts + 64 + b * 32, reinterpret_cast<const uint32_t(&)[32]>(lo[b * 32]));
         }
         float l0, l1;
         unpair(sum2, l0, l1);
         l += l0 + l1;
-        if (SPLIT) p_done(0);
-        p_done(1);
+        tmem_st_wait();
+        done(&c->p_full[w][1]);
       }
       // ---- out = O / l ----
       if (nk > 0 && ok) {
-        ok = wait_warp(&c->o_full[w], 0, c);
+        ok = wait_warp(&c->pv_done[w], (nk - 1) & 1, c);
         fence_after();
       }
       if (ok) {
@@ -530,7 +579,7 @@ __global__ void __launch_bounds__(TT, 1)
         // chunk i of a row at i ^ (row % 8).
         constexpr int ES = SPLIT ? 4 : 2, CH = HD * ES / 16;  // bytes of an output element, chunks of a row
         constexpr int X = CH < 8 ? CH - 1 : 7;
-        uint8_t* rows = qs + w * NS * C::TILE + wrow % TM * (HD * ES);
+        uint8_t* rows = qs + w * NS * C::QTILE + wrow % TM * (HD * ES);
         const float inv = 1.0f / l;
         bool finite = true;
 #pragma unroll 1
@@ -584,7 +633,7 @@ __global__ void __launch_bounds__(TT, 1)
       }
     }
   } else {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_OTHER));
   if (warp == 8 || warp == 10) {
     // ---- K tiles (warp 8) and V tiles (warp 10) ----
     const int v = warp == 10;
@@ -592,7 +641,8 @@ __global__ void __launch_bounds__(TT, 1)
     const int past_end = p.n_pages * p.n_head_kv * PG;  // a row outside the map: zeros
     const int* table = p.page_table + (int64_t)t.seq * p.max_pages;
     const int kv_end = t.past + t.n_q;  // keys of the sequence
-    // lane i: row in the map of page entry e + i, for the 32 entries (four tiles) from e
+    // lane i: row in the map of page entry e + i, for as many whole tiles as 32 lanes hold
+    constexpr int AHEAD = 32 / PPT;
     auto rows_from = [&](int e) {
       int y = past_end;
       if (e + lane < sp.n) {
@@ -602,99 +652,94 @@ __global__ void __launch_bounds__(TT, 1)
       }
       return y;
     };
-    int ahead = rows_from(0), y = past_end;
+    int ahead = rows_from(0), y = past_end, in = 0, slot = 0;
+    uint32_t use = 0;  // how often the slot was filled before
     bool ok = true;
-    int slot = v % C::STAGES;
-    uint32_t use = v / C::STAGES;  // how often the slot was filled before
     for (int n = 0; n < nk && ok; ++n) {
-      if (n % 4 == 0) {
+      if (in == 0) {
         y = ahead;
-        ahead = rows_from((n + 4) * PPT);
+        ahead = rows_from((n + AHEAD) * PPT);
       }
       // rows of the last page past the sequence's end
       const int n_tail = v && n == nk - 1 ? (sp.page(sp.n - 1) + 1) * PG - kv_end : 0;
-      if (use > 0 && !(ok = wait_warp(&c->empty[slot], (use - 1) & 1, c))) break;
-      uint64_t* bar = n_tail > 0 ? &c->tail : &c->full[slot];
+      if (use > 0 && !(ok = wait_warp(&c->empty[v][slot], (use - 1) & 1, c))) break;
+      uint64_t* bar = n_tail > 0 ? &c->tail : &c->full[v][slot];
       if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
       __syncwarp();
-      const uint32_t dst = smem_u32(ring + slot * C::TILE);
-      const int yy = __shfl_sync(0xffffffffu, y, n % 4 * PPT + lane % PPT);
+      uint8_t* tile = ring + (v * C::STAGES + slot) * C::TILE;
+      const int yy = __shfl_sync(0xffffffffu, y, in * PPT + lane % PPT);
       if (lane < PPT * C::HALVES)
-        tma_page(dst + (lane / PPT) * (TK * 128) + (lane % PPT) * (PG * 128), map, yy, bar, lane / PPT);
+        tma_page(smem_u32(tile) + (lane / PPT) * (TK * 128) + (lane % PPT) * (PG * 128), map, yy, bar, lane / PPT);
       __syncwarp();
       if (n_tail > 0) {
         ok = wait_warp(&c->tail, 0, c);
         const int key0 = (sp.n - 1 - n * PPT) * PG + PG - n_tail;
         for (int x = lane; x < n_tail * 8 * C::HALVES; x += 32) {
           const int key = key0 + x / 8 % n_tail, half = x / 8 / n_tail;
-          *reinterpret_cast<uint4*>(ring + slot * C::TILE + half * (TK * 128) + key * 128 + x % 8 * 16) =
-              make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(tile + half * (TK * 128) + key * 128 + x % 8 * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&c->full[slot]);
+        if (lane == 0) mbar_arrive(&c->full[v][slot]);
       }
-      if ((slot += 2) >= C::STAGES) slot -= C::STAGES, ++use;
+      if (++slot == C::STAGES) slot = 0, ++use;
+      if (++in == AHEAD) in = 0;
     }
-  } else if (warp == 9) {
-    // ---- products ----
-    constexpr uint32_t QK = idesc_f16(BF16, TK, 0), PV = idesc_f16(BF16, HDP, 1);
-    const uint32_t q_lo = desc_lo(smem_u32(qs), 16), k_lo = desc_lo(smem_u32(ring), 16);
-    const uint32_t v_lo = desc_lo(smem_u32(ring), TK * 128);
-    auto qk = [&](int w, int slot) {
-      const uint32_t a = q_lo + w * (NS * C::TILE >> 4), b = k_lo + slot * (C::TILE >> 4), d = tmem + w * 128;
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int k = 0; k < HDP / 16; ++k) {
-          const uint32_t off = ((k / 4) * (TM * 128) + (k % 4) * 32) >> 4;
-          mma_ss(d, a + (s * C::TILE >> 4) + off, b + off, QK, s + k > 0);
-        }
-    };
-    auto pv = [&](int w, int slot, int half, uint32_t acc) {
-      const uint32_t a = tmem + w * 128 + half * (TK / 4), b = v_lo + ((slot * C::TILE + half * (TK / 2) * 128) >> 4);
-      const uint32_t d = tmem + 256 + w * HDP;
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int k = 0; k < TK / 32; ++k) mma_ts(d, a + s * 64 + k * 8, b + (k * 2048 >> 4), PV, s + k > 0 ? 1 : acc);
-    };
-    if (elect_one()) {  // one thread for the whole loop: a vote or a warp barrier at each wait costs more than the wait
-      bool ok = nk > 0;
-      if (ok) ok = wait(&c->full[0], 0, c);
-      for (int w = 0; w < n_tiles && ok; ++w) {
-        if (!(ok = wait(&c->q_ready[w], 0, c))) break;
-        fence_after();
-        qk(w, 0);
-        commit(&c->s_full[w]);
-        if (w == n_tiles - 1) commit(&c->empty[0]);
-      }
-      int sv = 1 % C::STAGES, sk = 2 % C::STAGES;   // slots of V(n), K(n + 1) and their phases
-      uint32_t fv = 1 / C::STAGES, fk = 2 / C::STAGES;
+  } else if (elect_one()) {
+    // ---- products, one thread each: Q K^T (warp 9), P V (warp 11) ----
+    // One thread for a whole loop: a vote or a warp barrier at each wait would cost more than the wait.
+    if (warp == 9) {
+      constexpr uint32_t QK = idesc_f16(BF16, TK, 0);
+      const uint32_t q_lo = desc_lo(smem_u32(qs), 16), k_lo = desc_lo(smem_u32(ring), 16);
+      int slot = 0;
+      uint32_t use = 0;
+      bool ok = true;
       for (int n = 0; n < nk && ok; ++n) {
-        const bool more = n + 1 < nk;
-        if (!(ok = wait(&c->full[sv], fv & 1, c))) break;
-        if (more && !(ok = wait(&c->full[sk], fk & 1, c))) break;
+        if (!(ok = wait(&c->full[0][slot], use & 1, c))) break;
 #pragma unroll 1
         for (int w = 0; w < n_tiles; ++w) {
-          if (!(ok = wait(&c->p_full[w][0], n & 1, c))) break;
+          if (!(ok = n == 0 ? wait(&c->q_ready[w], 0, c) : wait(&c->s_free[w], (n - 1) & 1, c))) break;
           fence_after();
-          pv(w, sv, 0, n > 0);
-          if (!(ok = wait(&c->p_full[w][1], n & 1, c))) break;
-          fence_after();
-          pv(w, sv, 1, 1);
-          if (more) qk(w, sk);
-          commit(more ? &c->s_full[w] : &c->o_full[w]);
-          if (w == n_tiles - 1) {
-            commit(&c->empty[sv]);
-            if (more) commit(&c->empty[sk]);
-          }
+          const uint32_t a = q_lo + w * (NS * C::QTILE >> 4), b = k_lo + slot * (C::TILE >> 4), d = tmem + w * TK;
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = 0; k < HDP / 16; ++k)
+              mma_ss(d, a + ((s * C::QTILE + k / 4 * (TM * 128) + k % 4 * 32) >> 4),
+                     b + ((k / 4 * (TK * 128) + k % 4 * 32) >> 4), QK, s + k > 0);
+          commit(&c->s_full[w]);
+          if (w == n_tiles - 1) commit(&c->empty[0][slot]);
         }
-        if ((sv += 2) >= C::STAGES) sv -= C::STAGES, ++fv;
-        if ((sk += 2) >= C::STAGES) sk -= C::STAGES, ++fk;
+        if (++slot == C::STAGES) slot = 0, ++use;
+      }
+    } else if (warp == 11) {
+      constexpr uint32_t PV = idesc_f16(BF16, HDP, 1);
+      const uint32_t v_lo = desc_lo(smem_u32(ring + C::STAGES * C::TILE), TK * 128);
+      int slot = 0;
+      uint32_t use = 0;
+      bool ok = true;
+      for (int n = 0; n < nk && ok; ++n) {
+        if (!(ok = wait(&c->full[1][slot], use & 1, c))) break;
+#pragma unroll 1
+        for (int w = 0; w < n_tiles; ++w) {
+          const uint32_t a = tmem + C::P0 + w * C::PCOLS, b = v_lo + slot * (C::TILE >> 4), d = tmem + C::O0 + w * HDP;
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            if (!(ok = wait(&c->p_full[w][part], n & 1, c))) break;
+            fence_after();
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+              for (int k = part ? C::FIRST / 16 : 0; k < (part ? TK : C::FIRST) / 16; ++k)
+                mma_ts(d, a + s * (TK / 2) + k * 8, b + (k * 2048 >> 4), PV, part + s + k > 0 ? 1 : n > 0);
+          }
+          if (!ok) break;
+          commit(&c->pv_done[w]);
+          if (w == n_tiles - 1) commit(&c->empty[1][slot]);
+        }
+        if (++slot == C::STAGES) slot = 0, ++use;
       }
     }
-    __syncwarp();
   }
   }
   __syncwarp();
@@ -703,7 +748,7 @@ __global__ void __launch_bounds__(TT, 1)
   if (*(volatile int*)&c->abort) {
     if (tid == 0) report(p.status, ERR_TIMEOUT);
     // a wait ran out: the products and copies still under way end before the memory goes
-    if (warp == 9 && lane == 0) {
+    if ((warp == 9 || warp == 11) && elect_one()) {
       commit(&c->drain);
       for (int i = 0; i < 1 << 14 && !mbar_try_wait(&c->drain, 0); ++i) {
       }
