@@ -43,8 +43,7 @@ struct AppendParams {
   const int* pos;  // [n_tok]
   int* status;     // or null
   int vec;         // 16-byte accesses: bit 0 q, 1 k, 2 v, 3 q_out
-  int lpr;         // lanes per head row (a power of two, 8 elements each)
-  int tpc;         // tokens per CTA
+  int share;       // warps that share a token's heads
   uint8_t axis[APPEND_MAX_PAIRS];
 };
 cudaError_t launch_append(AppendParams& p, int io, int kv, int sm_count, cudaStream_t st);

@@ -6,170 +6,188 @@
 //   (a, b) -> (a cos - b sin, a sin + b cos)                pairs (2i, 2i+1) or (i, i + n_rot/2)
 //   q -> q_out; k, v -> row pos % 16 of page table[seq][pos / 16]
 //
-// Bound by memory: every element is read once and written once, a few
-// operations on each.  The angles of a token are the same for all of its
-// heads, so a CTA takes all heads of its tokens (or a share of them when
-// there are few tokens) and computes each cosine and sine once.  The angle is
-// formed and reduced in turns, in 64 bits: at position 1e5 an f32 product is
-// already off by up to 4e-3 radians, and the 64-bit product and subtraction
-// cost one thread per pair a few instructions.  A head row is spread over
-// hd / 8 lanes of one warp, 16 bytes each for 16-bit types, so the norm and
-// the partner of a half-split pair are warp shuffles.
+// Bound by memory: every element is read once and written once.  What stands in
+// the way is the arithmetic, so it is folded: with r the row's reciprocal norm and
+// y the partner of x, the weight and the rotation are
+//   out_e = r (x_e A_e + y_e B_e),  A_e = w_e cos, B_e = -+ w_partner sin
+// and A, B depend on the token alone.  A warp takes the heads of one token (or a
+// share of them when there are few tokens): it makes the token's table in shared
+// memory while its first rows are on their way, then walks the q, k and v heads, a
+// row on hd / 8 lanes, 16 bytes each for 16-bit types, with the next PF loads under
+// way.  The norm and the partner of a half-split pair are warp shuffles (of the
+// words as loaded).  No warp waits for another, every address is a constant step
+// from the last.  (A CTA to a token or several, rows dealt out by an index that
+// runs over tokens and heads: 262 instructions a step and 147 us where this takes
+// 66, 8192 tokens of 64 + 8 + 8 heads of 128 in bf16, both norms.)
+// The angle is formed and reduced in turns, in 64 bits: at position 1e5 an f32
+// product is already off by up to 4e-3 radians, and the 64-bit product and
+// subtraction cost one lane per pair a few instructions.
 #include "sfk_paged.cuh"
 
 namespace sfk {
 namespace {
 
-constexpr int AT = 256;  // threads
-constexpr int TPC_MAX = 16;
+constexpr int AW = 4;  // warps per CTA
+constexpr int PF = 4;  // loads ahead
 
-template <class IO, class KV, int P>
-__global__ void __launch_bounds__(AT) append_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ float2 cs[];  // [tpc][n_rot / 2] cosine, sine
-  __shared__ int s_pos[TPC_MAX], s_page[TPC_MAX];
-  const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * p.tpc;
-  const int nt = min(p.tpc, p.n_tok - t0);
-  const int rows = p.n_head + 2 * p.n_head_kv;
-  const int lpr = p.lpr, sub = tid & (lpr - 1), e0 = sub * 8;
-  const int rpp = AT / lpr;  // rows per pass
+// LPR: lanes per row (8 elements each)
+template <class IO, class KV, int LPR>
+__global__ void __launch_bounds__(AW * 32) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int R = 32 / LPR;  // rows per step
+  extern __shared__ __align__(16) float4 tables[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t item = (int64_t)blockIdx.x * AW + warp;
+  const int64_t t = item / p.share;
+  if (t >= p.n_tok) return;
+  const int sub = lane % LPR, e0 = sub * 8, rr = lane / LPR;
   const bool lane_on = e0 < p.hd;
+  const int nq = (p.n_head + R - 1) / R, nk = (p.n_head_kv + R - 1) / R, steps = nq + 2 * nk;
 
-  // 1. every row this thread takes is requested before anything waits
-  Raw8<IO> raw[P];
-  int tok[P], row[P];  // token within the CTA (-1: none), row within the token
+  const IO* qp = static_cast<const IO*>(p.q) + t * p.q_stride + rr * p.hd + e0;
+  const IO* kp = static_cast<const IO*>(p.k) + t * p.k_stride + rr * p.hd + e0;
+  const IO* vp = static_cast<const IO*>(p.v) + t * p.v_stride + rr * p.hd + e0;
+  auto load = [&](Raw8<IO>& raw, int i) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int slot = (i * gridDim.y + blockIdx.y) * rpp + tid / lpr;
-    tok[i] = slot < nt * rows ? slot / rows : -1;
-    row[i] = slot % rows;
-    if (tok[i] >= 0 && lane_on) {
-      const int64_t t = t0 + tok[i];
-      if (row[i] < p.n_head)
-        load8(raw[i], static_cast<const IO*>(p.q) + t * p.q_stride + (int64_t)row[i] * p.hd + e0, p.vec & 1);
-      else if (row[i] < p.n_head + p.n_head_kv)
-        load8(raw[i], static_cast<const IO*>(p.k) + t * p.k_stride + (int64_t)(row[i] - p.n_head) * p.hd + e0, p.vec & 2);
-      else
-        load8(raw[i], static_cast<const IO*>(p.v) + t * p.v_stride + (int64_t)(row[i] - p.n_head - p.n_head_kv) * p.hd + e0,
-              p.vec & 4);
+    for (int k = 0; k < (int)sizeof(IO) / 2; ++k) raw.w[k] = make_uint4(0, 0, 0, 0);
+    if (i < nq) {
+      if (lane_on && i * R + rr < p.n_head) load8(raw, qp + i * R * p.hd, p.vec & 1);
+    } else if (i < nq + nk) {
+      if (lane_on && (i - nq) * R + rr < p.n_head_kv) load8(raw, kp + (i - nq) * R * p.hd, p.vec & 2);
+    } else if (i < steps) {
+      if (lane_on && (i - nq - nk) * R + rr < p.n_head_kv) load8(raw, vp + (i - nq - nk) * R * p.hd, p.vec & 4);
     }
+  };
+  const int first = (int)(item % p.share);
+  Raw8<IO> next[PF];
+#pragma unroll
+  for (int k = 0; k < PF; ++k) load(next[k], first + k * p.share);
+
+  // the token's slot
+  const int pos = p.pos[t];
+  if (pos < 0) return;
+  const int sq = p.seq ? p.seq[t] : (int)t;
+  if (sq < 0 || sq >= p.n_seq || pos / PG >= p.max_pages) {
+    report(p.status, sq < 0 || sq >= p.n_seq ? ERR_BAD_ID : ERR_BAD_POS);
+    return;
   }
-  // 2. the slot of each token, and its angles
-  if (tid < nt) {
-    const int t = t0 + tid;
-    const int pos = p.pos[t];
-    const int s = p.seq ? p.seq[t] : t;
-    int page = -1, keep = pos;
-    if (pos >= 0) {
-      if (s < 0 || s >= p.n_seq) {
-        report(p.status, ERR_BAD_ID);
-        keep = -1;
-      } else if (pos / PG >= p.max_pages) {
-        report(p.status, ERR_BAD_POS);
-        keep = -1;
-      } else {
-        page = p.page_table[(int64_t)s * p.max_pages + pos / PG];
-        if (page < 0 || page >= p.n_pages) {
-          report(p.status, ERR_BAD_PAGE);
-          page = -1;
-        }
-      }
-    }
-    s_pos[tid] = keep;
-    s_page[tid] = page;
-  }
-  const int half = p.n_rot / 2;
-  for (int i = tid; i < nt * half; i += AT) {
-    const int t = t0 + i / half, c = i % half;
-    const int where = p.rope_pos ? p.rope_pos[(int64_t)p.axis[c] * p.n_tok + t] : p.pos[t];
+  const int page = p.page_table[(int64_t)sq * p.max_pages + pos / PG];
+  const bool page_ok = page >= 0 && page < p.n_pages;
+  if (!page_ok) report(p.status, ERR_BAD_PAGE);
+  // its table: (A, B) of element 8 i + j is float2 j % 2 of entry [j / 2][i], so that lanes read side by side
+  const int half = p.n_rot / 2, lanes = p.hd / 8;
+  const int kinds = p.q_norm == p.k_norm ? 1 : 2;
+  float4* table = tables + warp * kinds * p.hd / 2;
+  auto entry = [&](int k, int e) {
+    return reinterpret_cast<float2*>(table + k * p.hd / 2 + (e % 8 / 2) * lanes + e / 8) + e % 2;
+  };
+  for (int c = lane; c < half; c += 32) {
+    const int where = p.rope_pos ? p.rope_pos[(int64_t)p.axis[c] * p.n_tok + t] : pos;
     double turns = (double)where * (double)p.freqs[c] * 0.15915494309189533577;  // 1 / (2 pi)
     turns -= rint(turns);
-    float s, co;
-    sincospif(2.0f * (float)turns, &s, &co);
-    cs[i] = make_float2(co, s);
+    float sn, co;
+    sincospif(2.0f * (float)turns, &sn, &co);
+    const int a = p.neox ? c : 2 * c, b = p.neox ? c + half : 2 * c + 1;
+    for (int k = 0; k < kinds; ++k) {
+      const float* w = k ? p.k_norm : p.q_norm;
+      const float wa = w ? w[a] : 1.f, wb = w ? w[b] : 1.f;
+      *entry(k, a) = make_float2(wa * co, -wb * sn);
+      *entry(k, b) = make_float2(wb * co, wa * sn);
+    }
   }
-  __syncthreads();
-  // 3. norm, rotation, stores.  The lanes of a row agree on every branch.
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const bool mine = tok[i] >= 0 && s_pos[max(tok[i], 0)] >= 0;
-    const int tk = max(tok[i], 0);
-    float x[8];
-    if (mine && lane_on) {
-      unpack8(raw[i], x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  for (int e = p.n_rot + lane; e < p.hd; e += 32)
+    for (int k = 0; k < kinds; ++k) {
+      const float* w = k ? p.k_norm : p.q_norm;
+      *entry(k, e) = make_float2(w ? w[e] : 1.f, 0.f);
     }
-    const bool is_q = row[i] < p.n_head, is_v = row[i] >= p.n_head + p.n_head_kv;
-    const float* w = is_v ? nullptr : (is_q ? p.q_norm : p.k_norm);
-    if (p.q_norm || p.k_norm) {
-      float ss = 0.f;
+  __syncwarp();
+
+  const float inv_hd = 1.0f / (float)p.hd;
+  const bool turned = e0 < p.n_rot;  // past n_rot the partner, whatever it is, has no part
+  // e0 .. e0+7 is wholly in the first or the second half (half % 8 == 0)
+  const int from = (e0 < half ? sub + half / 8 : sub - half / 8) & (LPR - 1);
+  IO* op = static_cast<IO*>(p.q_out) + t * p.out_stride + rr * p.hd + e0;
+  const int64_t at = (((int64_t)page * p.n_head_kv + rr) * PG + pos % PG) * p.hd + e0;
+  KV* kd = static_cast<KV*>(p.k_pages) + at;
+  KV* vd = static_cast<KV*>(p.v_pages) + at;
+  for (int i0 = first; i0 < steps; i0 += PF * p.share) {
+    Raw8<IO> raw[PF];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-      for (int o = lpr / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (w && lane_on) {
-        const float r = 1.0f / sqrtf(ss / (float)p.hd + p.eps);
+    for (int k = 0; k < PF; ++k) raw[k] = next[k];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e0 + e];
+    for (int k = 0; k < PF; ++k) load(next[k], i0 + (PF + k) * p.share);
+#pragma unroll
+    for (int k = 0; k < PF; ++k) {
+      const int i = i0 + k * p.share;
+      if (i >= steps) break;
+      float x[8];
+      unpack8(raw[k], x);
+      if (i >= nq + nk) {  // v: as it is
+        const int h = (i - nq - nk) * R;
+        if (lane_on && page_ok && h + rr < p.n_head_kv) store8(vd + (int64_t)h * PG * p.hd, x, true);
+        continue;
       }
-    }
-    if (p.n_rot > 0) {
-      const float2* a = cs + tk * half;
-      if (p.neox) {
-        // e0 .. e0+7 is wholly in the first or the second half (half % 8 == 0)
-        const bool lo = e0 < half;
-        const int d = half / 8;
-        const int from = (lo ? sub + d : sub - d) & (lpr - 1);
-        float y[8];
+      const bool is_q = i < nq;
+      float r = 1.f;
+      if (is_q ? p.q_norm != nullptr : p.k_norm != nullptr) {
+        float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from, lpr);
-        if (!is_v && mine && e0 < p.n_rot) {
-          const float2* ae = a + (lo ? e0 : e0 - half);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = lo ? x[e] * ae[e].x - y[e] * ae[e].y : y[e] * ae[e].y + x[e] * ae[e].x;
-        }
-      } else if (!is_v && mine && e0 < p.n_rot) {
-        const float2* ae = a + e0 / 2;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = x[2 * e], v = x[2 * e + 1];
-          x[2 * e] = u * ae[e].x - v * ae[e].y;
-          x[2 * e + 1] = u * ae[e].y + v * ae[e].x;
-        }
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        r = rsqrtf(fmaf(ss, inv_hd, p.eps));
       }
-    }
-    if (!mine || !lane_on) continue;
-    const int64_t t = t0 + tk;
-    if (is_q) {
-      store8(static_cast<IO*>(p.q_out) + t * p.out_stride + (int64_t)row[i] * p.hd + e0, x, p.vec & 8);
-    } else if (s_page[tk] >= 0) {
-      const int h = row[i] - p.n_head - (is_v ? p.n_head_kv : 0);
-      KV* base = static_cast<KV*>(is_v ? p.v_pages : p.k_pages);
-      store8(base + (((int64_t)s_page[tk] * p.n_head_kv + h) * PG + s_pos[tk] % PG) * p.hd + e0, x, true);
+      float y[8];  // partners
+      if (p.neox && half > 0) {
+        Raw8<IO> other;
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(IO) / 2; ++j) {
+          other.w[j].x = __shfl_sync(0xffffffffu, raw[k].w[j].x, from, LPR);
+          other.w[j].y = __shfl_sync(0xffffffffu, raw[k].w[j].y, from, LPR);
+          other.w[j].z = __shfl_sync(0xffffffffu, raw[k].w[j].z, from, LPR);
+          other.w[j].w = __shfl_sync(0xffffffffu, raw[k].w[j].w, from, LPR);
+        }
+        unpack8(other, y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+      }
+      if (!lane_on) continue;
+      const float4* ab = table + (is_q ? 0 : kinds - 1) * p.hd / 2 + sub;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 z = ab[e * lanes];
+        x[2 * e] *= z.x;
+        x[2 * e + 1] *= z.z;
+        if (turned) {
+          x[2 * e] = fmaf(y[2 * e], z.y, x[2 * e]);
+          x[2 * e + 1] = fmaf(y[2 * e + 1], z.w, x[2 * e + 1]);
+        }
+        x[2 * e] *= r;
+        x[2 * e + 1] *= r;
+      }
+      if (is_q) {
+        if (i * R + rr < p.n_head) store8(op + i * R * p.hd, x, p.vec & 8);
+      } else {
+        const int h = (i - nq) * R;
+        if (page_ok && h + rr < p.n_head_kv) store8(kd + (int64_t)h * PG * p.hd, x, true);
+      }
     }
   }
 }
 
 template <class IO, class KV>
 cudaError_t launch_t(AppendParams& p, int sm_count, cudaStream_t st) {
-  const int rows = p.n_head + 2 * p.n_head_kv;
-  p.lpr = 1;
-  while (p.lpr * 8 < p.hd) p.lpr *= 2;
-  const int rpp = AT / p.lpr;
-  // Few rows per token: several tokens to a CTA, as long as every SM has work
-  p.tpc = 1;
-  while (p.tpc < TPC_MAX && (p.tpc + 1) * rows <= 2 * rpp && (int64_t)p.n_tok > (int64_t)(p.tpc + 1) * 4 * sm_count) ++p.tpc;
-  const int passes = (p.tpc * rows + rpp - 1) / rpp;
-  const int64_t groups = (p.n_tok + p.tpc - 1) / p.tpc;
-  // Many tokens: up to four rows per thread in flight; few: one pass per CTA,
-  // so that the heads of a token spread over the SMs.
-  const int P = groups * passes <= 4 * sm_count ? 1 : (passes >= 3 ? 4 : passes);
-  const dim3 grid((unsigned)groups, (unsigned)((passes + P - 1) / P));
-  const size_t smem = sizeof(float2) * p.tpc * (p.n_rot / 2);
-  if (P == 1) append_kernel<IO, KV, 1><<<grid, AT, smem, st>>>(p);
-  else if (P == 2) append_kernel<IO, KV, 2><<<grid, AT, smem, st>>>(p);
-  else append_kernel<IO, KV, 4><<<grid, AT, smem, st>>>(p);
+  const int lpr = p.hd <= 32 ? 4 : p.hd <= 64 ? 8 : p.hd <= 128 ? 16 : 32;
+  const int R = 32 / lpr, steps = (p.n_head + R - 1) / R + 2 * ((p.n_head_kv + R - 1) / R);
+  // warps per token: enough for 32 warps on every SM, a step each at least
+  p.share = 1;
+  while (p.share < steps && (int64_t)p.n_tok * p.share < (int64_t)32 * sm_count) ++p.share;
+  const int64_t ctas = ((int64_t)p.n_tok * p.share + AW - 1) / AW;
+  const size_t smem = (size_t)AW * (p.q_norm == p.k_norm ? 1 : 2) * p.hd * sizeof(float2);
+  if (lpr == 4) append_kernel<IO, KV, 4><<<(unsigned)ctas, AW * 32, smem, st>>>(p);
+  else if (lpr == 8) append_kernel<IO, KV, 8><<<(unsigned)ctas, AW * 32, smem, st>>>(p);
+  else if (lpr == 16) append_kernel<IO, KV, 16><<<(unsigned)ctas, AW * 32, smem, st>>>(p);
+  else append_kernel<IO, KV, 32><<<(unsigned)ctas, AW * 32, smem, st>>>(p);
   return cudaGetLastError();
 }
 
