@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "sfk_device.cuh"
 
@@ -116,20 +117,48 @@ __device__ __forceinline__ void load8(Raw8<T>& r, const T* p, bool vec) {
 }
 template <class T>
 __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&x)[8]) {
-  const T* e = reinterpret_cast<const T*>(r.w);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
 }
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8], bool vec) {
   Raw8<T> r;
-  T* e = reinterpret_cast<T*>(r.w);
+  uint32_t* w = reinterpret_cast<uint32_t*>(r.w);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        const __half2 v = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+  }
   if (vec) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
   } else {
+    const T* e = reinterpret_cast<const T*>(r.w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = e[i];
   }
@@ -151,6 +180,32 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// ---- two f32 at a time ----------------------------------------------------------
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float x) { return pair(x, x); }
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 __device__ __forceinline__ void report(int* status, int code) {
