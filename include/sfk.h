@@ -564,7 +564,8 @@ SFK_API sfk_status sfk_attn_decode_window(int32_t io_type, const void *dev_q, in
                                           void *stream);
 /* Bytes of workspace with which that call is fastest (0: it uses none; it
  * depends on the sizes and the current device alone). */
-SFK_API size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t head_dim);
+SFK_API size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                                                int32_t max_pages, int32_t window, int32_t n_sink);
 
 /* The same attention for the newest tokens of each of n_seq sequences: rows
  * q_start[s] .. q_start[s+1]-1 of q (q_start [n_seq + 1], ascending, device)

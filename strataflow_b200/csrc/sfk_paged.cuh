@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -74,11 +75,25 @@ struct WindowAttnParams {
 };
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
 // p.partial / p.ws_bytes: the caller's workspace, or null
-size_t window_decode_workspace(int64_t n_seq, int n_head, int n_head_kv, int hd, int sm_count);
+size_t window_decode_workspace(const WindowAttnParams& p, int hd, int sm_count);
 cudaError_t launch_window_prefill(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
 // the tensor-core form: whether it takes these types and sizes, and its launch
 bool prefill_tc_takes(const WindowAttnParams& p, int kv, int hd);
 cudaError_t launch_prefill_tc(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
+
+// Dynamic shared memory above 48 KB has to be allowed once per kernel and device (two threads may do it twice).
+template <auto Kernel>
+inline cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 #ifdef __CUDACC__
 // ---- element access -----------------------------------------------------------

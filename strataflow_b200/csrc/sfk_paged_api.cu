@@ -178,9 +178,19 @@ sfk_status sfk_attn_decode_window(int32_t io_type, const void* q, int64_t q_stri
   return cuda_result(launch_window_decode(a, kv, hd, current_sms(), (cudaStream_t)stream), who);
 }
 
-size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t hd) {
-  if (n_seq < 1 || n_head < 1 || n_head_kv < 1 || n_head % n_head_kv || hd < 1 || hd > 256) return 0;
-  return window_decode_workspace(n_seq, n_head, n_head_kv, hd, current_sms());
+size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t hd, int32_t max_pages,
+                                        int32_t window, int32_t n_sink) {
+  if (n_seq < 1 || n_seq > 65535 || n_head < 1 || n_head_kv < 1 || n_head % n_head_kv || hd < 1 || hd > 256 ||
+      max_pages < 1 || max_pages > MAX_PAGES || window < 0 || n_sink < 0)
+    return 0;
+  WindowAttnParams a{};
+  a.n_seq = n_seq;
+  a.n_head = n_head;
+  a.n_head_kv = n_head_kv;
+  a.max_pages = max_pages;
+  a.window = window;
+  a.n_sink = n_sink;
+  return window_decode_workspace(a, hd, current_sms());
 }
 
 sfk_status sfk_attn_prefill_window(int32_t io_type, const void* q, int64_t q_stride, int32_t n_tok, int32_t kv_type,

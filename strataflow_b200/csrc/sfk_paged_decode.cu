@@ -612,10 +612,10 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
   join_and_store(sm.join, p, w.seq, w.head0, w.n_rows, w.pos >= 0);
 }
 
-template <class K, class... Maps>
-cudaError_t launch_parts(K kernel, const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st,
+template <auto Kernel, class... Maps>
+cudaError_t launch_parts(const WindowAttnParams& p, int tiles, int threads, size_t smem, cudaStream_t st,
                          const Maps&... maps) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<Kernel>(smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.n_head_kv * tiles * p.parts), (unsigned)p.n_seq);
@@ -628,7 +628,7 @@ cudaError_t launch_parts(K kernel, const WindowAttnParams& p, int tiles, int thr
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p, maps...);
+  return cudaLaunchKernelEx(&cfg, Kernel, p, maps...);
 }
 
 template <int HD>
@@ -662,20 +662,28 @@ int row_tiles(const WindowAttnParams& p) { return (p.n_head / p.n_head_kv + DEC_
 // walk more than LONG pages that way, the pages are split into one wave of `occ`
 // CTAs per SM, joined through the workspace.
 constexpr int LONG = 2;
-void pick_parts(WindowAttnParams& p, int occ, int hd, int sm_count) {
+struct Parts {
+  int cluster;    // CTAs per cluster without a workspace
+  int64_t split;  // CTAs with one, 0: not worth it
+  size_t bytes;   // the workspace
+};
+Parts count_parts(const WindowAttnParams& p, int occ, int hd, int sm_count) {
   const int64_t pages = max_seen_pages(p), pairs = (int64_t)p.n_seq * p.n_head_kv * row_tiles(p);
-  int c = 1;
-  while (c < 8 && pairs * c < 2 * sm_count && pages > (int64_t)c * DEC_W) c *= 2;
-  p.parts = c;
-  float* ws = p.partial;
-  p.partial = nullptr;
+  Parts r{1, 0, 0};
+  while (r.cluster < 8 && pairs * r.cluster < 2 * sm_count && pages > (int64_t)r.cluster * DEC_W) r.cluster *= 2;
   int64_t n = occ * sm_count / pairs;
   n = n < pages / (2 * DEC_W) ? n : pages / (2 * DEC_W);
-  if (n > 1 && pages > (int64_t)c * DEC_W * LONG && ws &&
-      p.ws_bytes >= (size_t)(n * p.n_seq * p.n_head * (hd + 2)) * sizeof(float)) {
-    p.parts = (int)n;
-    p.partial = ws;
+  if (n > 1 && pages > (int64_t)r.cluster * DEC_W * LONG) {
+    r.split = n;
+    r.bytes = (size_t)(n * p.n_seq * p.n_head * (hd + 2)) * sizeof(float);
   }
+  return r;
+}
+void pick_parts(WindowAttnParams& p, int occ, int hd, int sm_count) {
+  const Parts r = count_parts(p, occ, hd, sm_count);
+  const bool split = r.split && p.partial && p.ws_bytes >= r.bytes;
+  p.parts = split ? (int)r.split : r.cluster;
+  if (!split) p.partial = nullptr;
 }
 
 template <class KV, int HD>
@@ -683,7 +691,7 @@ cudaError_t launch_cc(WindowAttnParams& p, int sm_count, cudaStream_t st) {
   using Smem = CcSmem<KV, HD>;
   static_assert(Smem::R == DEC_R && Smem::DW == DEC_W, "pick_parts counts these");
   pick_parts(p, 2, HD, sm_count);
-  return launch_parts(decode_cc_kernel<KV, HD>, p, row_tiles(p), DEC_W * 32, sizeof(Smem), st);
+  return launch_parts<decode_cc_kernel<KV, HD>>(p, row_tiles(p), DEC_W * 32, sizeof(Smem), st);
 }
 
 template <class KV, int HD, bool SPLIT>
@@ -695,7 +703,8 @@ cudaError_t launch_mma(WindowAttnParams& p, int kv, int sm_count, cudaStream_t s
   if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, (HD + 63) / 64);
   if (e != cudaSuccess) return e;
   pick_parts(p, HD <= 128 ? 3 : 1, HD, sm_count);
-  return launch_parts(decode_mma_kernel<KV, HD, SPLIT, DEC_W>, p, row_tiles(p), DEC_W * 32, sizeof(Smem) + 1024, st, km, vm);
+  return launch_parts<decode_mma_kernel<KV, HD, SPLIT, DEC_W>>(p, row_tiles(p), DEC_W * 32, sizeof(Smem) + 1024, st, km,
+                                                               vm);
 }
 template <class KV, int HD>
 cudaError_t launch_16(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
@@ -716,10 +725,9 @@ cudaError_t launch_hd(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st
 
 }  // namespace
 
-size_t window_decode_workspace(int64_t n_seq, int n_head, int n_head_kv, int hd, int sm_count) {
-  // at most three CTAs for every SM write 8 heads each; none where one for each part of the batch fills that
-  const int64_t pairs = n_seq * n_head_kv * ((n_head / n_head_kv + DEC_R - 1) / DEC_R);
-  return pairs * 2 <= 3 * sm_count ? (size_t)3 * sm_count * DEC_R * (hd + 2) * sizeof(float) : 0;
+size_t window_decode_workspace(const WindowAttnParams& p, int hd, int sm_count) {
+  // of the kernel with the most CTAs per SM, and so the most parts
+  return count_parts(p, 3, hd, sm_count).bytes;
 }
 
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {

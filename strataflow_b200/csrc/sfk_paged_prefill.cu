@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__
 template <class KV, int HD>
 cudaError_t launch_fma(WindowAttnParams& p, cudaStream_t st) {
   const size_t smem = sizeof(FmaSmem<HD>);
-  cudaError_t e = cudaFuncSetAttribute(prefill_fma_kernel<KV, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<prefill_fma_kernel<KV, HD>>(smem);
   if (e != cudaSuccess) return e;
   const int64_t group = p.n_head / p.n_head_kv;
   const dim3 grid((unsigned)(p.n_tok * group / FR + p.n_seq), (unsigned)p.n_head_kv);

@@ -753,12 +753,11 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, cudaStream_t st) {
   cudaError_t e = pool_map(&km, p.k_pages, kv, HD, rows, 1);
   if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, 1);
   if (e != cudaSuccess) return e;
-  const auto kernel = prefill_tc_kernel<KV, HD, SPLIT>;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  e = allow_smem<prefill_tc_kernel<KV, HD, SPLIT>>(C::SMEM);
   if (e != cudaSuccess) return e;
   const int64_t group = p.n_head / p.n_head_kv;
   const int64_t tiles = p.n_tok * group / TC_ROWS + p.n_seq;
-  kernel<<<(unsigned)(tiles * p.n_head_kv), TT, C::SMEM, st>>>(p, km, vm);
+  prefill_tc_kernel<KV, HD, SPLIT><<<(unsigned)(tiles * p.n_head_kv), TT, C::SMEM, st>>>(p, km, vm);
   return cudaGetLastError();
 }
 

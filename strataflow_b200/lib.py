@@ -97,7 +97,7 @@ _SIGS = {
                                       P, I32, P, P, I32, P, I32, I32, P, P, P, I64, P, P]),
     "sfk_attn_decode_window": (I32, [I32, P, I64, I32, P, P, I32, P, I32, P, I32, I32, I32, I32, F, I32, I32, P, P,
                                      SZ, P, P]),
-    "sfk_attn_decode_window_workspace": (SZ, [I32, I32, I32, I32]),
+    "sfk_attn_decode_window_workspace": (SZ, [I32, I32, I32, I32, I32, I32, I32]),
     "sfk_attn_prefill_window": (I32, [I32, P, I64, I32, I32, P, P, I32, P, I32, P, P, I32, I32, I32, I32, F, I32, I32,
                                       P, P, P]),
     "sfk_device_status": (I32, [P, P]),

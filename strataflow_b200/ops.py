@@ -143,69 +143,74 @@ def _refuse(msg: str):
     raise L.SfkError(L.SFK_ERR_INVALID_ARGUMENT, msg)
 
 
-def _rows(t: torch.Tensor, what: str, heads: int, hd: int, dtype, device) -> tuple[int, int]:
+def _rows(t: torch.Tensor, what: str, heads: int, hd: int, dtype, dev: int) -> tuple[int, int]:
     """Pointer and token stride of [tokens][heads][hd] rows whose heads are contiguous."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.dtype != dtype or t.device != device:
-        _refuse(f"{what}: {dtype} [tokens][{heads}][{hd}] on {device} is wanted, got {t.dtype} {tuple(t.shape)} on "
+    shape, s = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hd or t.dtype is not dtype or t.get_device() != dev:
+        _refuse(f"{what}: {dtype} [tokens][{heads}][{hd}] on cuda:{dev} is wanted, got {t.dtype} {tuple(shape)} on "
                 f"{t.device}")
-    s = t.stride()
-    if (s[2] != 1 and hd > 1) or (s[1] != hd and heads > 1):
+    if s[2] != 1 or (s[1] != hd and heads > 1):
         _refuse(f"{what}: a token's heads have to be contiguous, got strides {s}")
-    return t.data_ptr(), (s[0] if t.shape[0] > 1 else max(s[0], heads * hd))
+    return t.data_ptr(), (s[0] if shape[0] > 1 else max(s[0], heads * hd))
 
 
-def _int32(t: torch.Tensor, what: str, shape, device) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        _refuse(f"{what}: contiguous int32 {list(shape)} on {device} is wanted, got {t.dtype} {list(t.shape)} on "
+def _plain(t: torch.Tensor, what: str, dtype, shape, dev: int) -> int:
+    """Pointer of a contiguous tensor of that type and shape."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{what}: contiguous {dtype} {list(shape)} on cuda:{dev} is wanted, got {t.dtype} {list(t.shape)} on "
                 f"{t.device}")
     return t.data_ptr()
 
 
-def _f32(t: torch.Tensor | None, what: str, n: int, device) -> int | None:
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        _refuse(f"{what}: contiguous float32 [{n}] on {device} is wanted, got {t.dtype} {list(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _int32(t: torch.Tensor, what: str, shape, dev: int) -> int:
+    return _plain(t, what, torch.int32, shape, dev)
 
 
-def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, device) -> tuple[int, int, int]:
+def _f32(t: torch.Tensor | None, what: str, n: int, dev: int) -> int | None:
+    return None if t is None else _plain(t, what, torch.float32, (n,), dev)
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, dev: int) -> tuple[int, int, int]:
     """(kv type, kv heads, head_dim) of a checked cache."""
-    if (k_pages.dim() != 4 or k_pages.shape[2] != 16 or k_pages.shape != v_pages.shape or
-            k_pages.dtype != v_pages.dtype or k_pages.dtype not in _KV_TYPES):
+    shape, kvt = k_pages.shape, _KV_TYPES.get(k_pages.dtype)
+    if len(shape) != 4 or shape[2] != 16 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or kvt is None:
         _refuse(f"page pools: two [n_pages][n_head_kv][16][head_dim] of one type (f32, f16, bf16) are wanted, got "
                 f"{k_pages.dtype} {tuple(k_pages.shape)} and {v_pages.dtype} {tuple(v_pages.shape)}")
-    if not (k_pages.is_contiguous() and v_pages.is_contiguous()) or k_pages.device != device or v_pages.device != device:
-        _refuse(f"page pools: contiguous and on {device}")
+    if (not (k_pages.is_contiguous() and v_pages.is_contiguous()) or k_pages.get_device() != dev or
+            v_pages.get_device() != dev):
+        _refuse(f"page pools: contiguous and on cuda:{dev}")
     if page_table.dim() != 2:
         _refuse("page_table: [n_seq][max_pages] is wanted")
-    return _KV_TYPES[k_pages.dtype], k_pages.shape[1], k_pages.shape[3]
+    return kvt, shape[1], shape[3]
 
 
-def _cuda_device(t: torch.Tensor, what: str):
-    if not t.is_cuda:
+def _cuda_device(t: torch.Tensor, what: str) -> int:
+    dev = t.get_device()
+    if dev < 0:
         _refuse(f"{what}: a CUDA tensor is wanted, got one on {t.device}")
-    return t.device
+    return dev
 
 
-def _call(device, fn, *args) -> None:
-    """Run an entry on `device`'s current stream (the library launches on the current device)."""
-    if device.index == torch.cuda.current_device():
-        L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+def _call(dev: int, fn, *args) -> None:
+    """Run an entry on device `dev`'s current stream (the library launches on the current device)."""
+    if dev == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(device):
-            L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        L.check(status)
 
 
-def _status(status: torch.Tensor | None, device) -> int | None:
-    return None if status is None else _int32(status, "status", (1,), device)
+def _status(status: torch.Tensor | None, dev: int) -> int | None:
+    return None if status is None else _int32(status, "status", (1,), dev)
 
 
 def check_status(status: torch.Tensor) -> None:
     """Wait for the current stream; raise SfkError if the status word of earlier
     paged-cache calls records an error, and clear it."""
-    device = _cuda_device(status, "status")
-    _call(device, L.load().sfk_device_status, _status(status, device))
+    dev = _cuda_device(status, "status")
+    _call(dev, L.load().sfk_device_status, _status(status, dev))
 
 
 def rope_freqs(n_rot: int, base: float = 10000.0, scale: float = 1.0, device="cuda") -> torch.Tensor:
@@ -251,7 +256,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     if k.shape[0] != n or v.shape[0] != n:
         _refuse(f"q, k and v: {n}, {k.shape[0]} and {v.shape[0]} tokens")
     if out is None:
-        out = torch.empty((n, heads, hd), dtype=q.dtype, device=dev)
+        out = q.new_empty((n, heads, hd))
     op, os_ = _rows(out, "out", heads, hd, q.dtype, dev)
     if out.shape[0] != n:
         _refuse(f"out: {n} tokens are wanted, got {out.shape[0]}")
@@ -285,16 +290,15 @@ def _attn_rows(q: torch.Tensor, k_pages: torch.Tensor, kvh: int, hd: int, window
     qp, qs = _rows(q, "q", heads, hd, q.dtype, dev)
     shape = (q.shape[0], heads * hd)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or tuple(out.shape) != shape or out.device != dev or not out.is_contiguous():
-        _refuse(f"out: contiguous {q.dtype} {list(shape)} on {dev} is wanted")
-    return heads, qp, qs, out
+        out = q.new_empty(shape)
+        return heads, qp, qs, out, out.data_ptr()
+    return heads, qp, qs, out, _plain(out, "out", q.dtype, shape, dev)
 
 
 @functools.lru_cache(maxsize=4096)
-def _decode_workspace(n_seq: int, heads: int, kvh: int, hd: int, device: int) -> int:
-    with torch.cuda.device(device):
-        return int(L.load().sfk_attn_decode_window_workspace(n_seq, heads, kvh, hd))
+def _decode_workspace(dev: int, *sizes: int) -> int:
+    with torch.cuda.device(dev):
+        return int(L.load().sfk_attn_decode_window_workspace(*sizes))
 
 
 def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -305,14 +309,14 @@ def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     with window > 0, j > p - window or j < n_sink.  Returns [n_seq][Hq * hd]."""
     dev = _cuda_device(q, "q")
     kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
-    heads, qp, qs, out = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
+    heads, qp, qs, out, op = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
     n = q.shape[0]
-    ws_bytes = _decode_workspace(n, heads, kvh, hd, dev.index)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    ws_bytes = _decode_workspace(dev, n, heads, kvh, hd, page_table.shape[1], window, n_sink)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _call(dev, L.load().sfk_attn_decode_window, _ROW_TYPES[q.dtype], qp, qs, kvt, k_pages.data_ptr(),
           v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
           page_table.shape[1], _int32(positions, "positions", (n,), dev), n, heads, kvh, hd, scale, window, n_sink,
-          out.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, _status(status, dev))
+          op, None if ws is None else ws.data_ptr(), ws_bytes, _status(status, dev))
     return out
 
 
@@ -326,10 +330,10 @@ def attn_prefill_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     Returns [tokens][Hq * hd]; rows of no sequence are not written."""
     dev = _cuda_device(q, "q")
     kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
-    heads, qp, qs, out = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
+    heads, qp, qs, out, op = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
     n = page_table.shape[0]
     _call(dev, L.load().sfk_attn_prefill_window, _ROW_TYPES[q.dtype], qp, qs, q.shape[0], kvt, k_pages.data_ptr(),
           v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
           page_table.shape[1], _int32(q_start, "q_start", (n + 1,), dev), _int32(kv_len, "kv_len", (n,), dev), n, heads,
-          kvh, hd, scale, window, n_sink, out.data_ptr(), _status(status, dev))
+          kvh, hd, scale, window, n_sink, op, _status(status, dev))
     return out

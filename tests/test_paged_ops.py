@@ -84,6 +84,15 @@ def test_empty_calls_do_nothing(sfk):
     assert call(sfk, "sfk_attn_prefill_window", PREFILL, n_tok=0, q=None) == L.SFK_OK
 
 
+def test_decode_workspace(sfk):
+    """Asked for where a small batch reads a long context, refused sizes need none."""
+    f = sfk.sfk_attn_decode_window_workspace
+    assert f(1, 32, 8, 128, 2048, 0, 0) > 0
+    assert f(1, 32, 8, 128, 2048, 256, 4) == 0 and f(1, 32, 8, 128, 16, 0, 0) == 0  # a short context
+    assert f(64, 32, 8, 128, 2048, 0, 0) == 0                                       # a batch that fills the GPU
+    assert f(0, 32, 8, 128, 2048, 0, 0) == 0 and f(1, 31, 8, 128, 2048, 0, 0) == 0 and f(1, 32, 8, 128, 0, 0, 0) == 0
+
+
 def test_device_status_needs_a_word(sfk):
     assert sfk.sfk_device_status(None, None) == L.SFK_ERR_INVALID_ARGUMENT
 
