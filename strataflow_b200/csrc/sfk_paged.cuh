@@ -72,6 +72,8 @@ struct WindowAttnParams {
   const int* q_start;  // [n_seq + 1]
   const int* kv_len;   // [n_seq]
   int n_tok;
+  int tile_rows;   // rows per CTA (tensor-core form)
+  int key_parts;   // CTAs of a cluster that share a row tile's keys (tensor-core form)
 };
 cudaError_t launch_window_decode(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st);
 // p.partial / p.ws_bytes: the caller's workspace, or null
@@ -258,8 +260,7 @@ struct Tile {
   int seq, q0, n_q, row0;  // first token of the sequence, its tokens, first row
   int past;                // position of its first token
 };
-template <int RT>
-__device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx) {
+__device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx, int RT) {
   const int lane = threadIdx.x & 31;
   const int64_t group = p.n_head / p.n_head_kv;
   Tile t;

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
   const int hk = blockIdx.y, G = p.n_head / p.n_head_kv;
-  const Tile t = find_tile<FR>(p, blockIdx.x);
+  const Tile t = find_tile(p, blockIdx.x, FR);
   if (t.seq < 0) return;
   const int n_rows = (int)min((int64_t)FR, (int64_t)t.n_q * G - t.row0);
   for (int i = tid; i < FR * HD; i += FT) {

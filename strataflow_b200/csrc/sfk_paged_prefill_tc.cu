@@ -26,8 +26,8 @@
 //
 // 32-bit rows over an f16 cache (SPLIT): q, scaled by a power of two per row,
 // is the sum of two f16 numbers and so is each P (22 bits), and each product
-// is two.  P is held up to 2^15 so that its second part stays above f16's
-// smallest step.  A bf16 pair holds 16 bits only: that cache takes the
+// is two.  P is 2^11 at m and 2^15 at most, so that its second part stays above
+// f16's smallest step.  A bf16 pair holds 16 bits only: that cache takes the
 // CUDA-core kernel.
 //
 // What a masked place holds does not matter: K only reaches its own column of
@@ -35,6 +35,8 @@
 // memory; a V row that some rows of a tile see and others do not reaches the
 // others as 0 * v, which is NaN for an infinite v: rows whose output is not
 // finite are computed again key by key (recompute_row).
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "sfk_paged.cuh"
@@ -42,6 +44,8 @@
 
 namespace sfk {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int TM = 128;       // rows per tile
 constexpr int TC_ROWS = 256;  // rows per CTA
@@ -323,17 +327,20 @@ __global__ void __launch_bounds__(TT, 1)
   uint8_t* ring = base + C::QB;         // [K, V][stage][half][TK keys][128 B]
   Ctl* c = reinterpret_cast<Ctl*>(base + C::QB + 2 * C::STAGES * C::TILE);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int G = p.n_head / p.n_head_kv, hk = blockIdx.x % p.n_head_kv;
+  const int parts = p.key_parts, part = blockIdx.x % parts, job = blockIdx.x / parts;
+  const int G = p.n_head / p.n_head_kv, hk = job % p.n_head_kv;
 
-  const Tile t = find_tile<TC_ROWS>(p, blockIdx.x / p.n_head_kv);
-  if (t.seq < 0) return;  // the whole CTA
-  const int n_rows = (int)min((int64_t)TC_ROWS, (int64_t)t.n_q * G - t.row0);
+  const Tile t = find_tile(p, job / p.n_head_kv, p.tile_rows);
+  if (t.seq < 0) return;  // the whole cluster
+  const int n_rows = (int)min((int64_t)p.tile_rows, (int64_t)t.n_q * G - t.row0);
   const int n_tiles = n_rows > TM ? 2 : 1;
   const int p_lo = max(t.past + t.row0 / G, 0), p_hi = t.past + (t.row0 + n_rows - 1) / G;
   SeenPages sp;
   sp.n = sp.sink = sp.first = 0;
   if (p_hi >= 0) sp = seen_pages(p_lo, p_hi, p.window, p.n_sink);
-  const int nk = (sp.n + PPT - 1) / PPT;
+  // this CTA's key tiles: n_first .. n_first + nk - 1 of n_all
+  const int n_all = (sp.n + PPT - 1) / PPT;
+  const int n_first = (int)((int64_t)n_all * part / parts), nk = (int)((int64_t)n_all * (part + 1) / parts) - n_first;
 
   if (tid == 0) {
     for (int v = 0; v < 2; ++v)
@@ -363,6 +370,8 @@ __global__ void __launch_bounds__(TT, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = c->tmem;
+  float* stage = reinterpret_cast<float*>(base);                // [256][HD]: a part's O
+  float2* ml = reinterpret_cast<float2*>(stage + TC_ROWS * HD);  // [256]: its m and l
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFTMAX));
@@ -451,8 +460,8 @@ __global__ void __launch_bounds__(TT, 1)
       }
       const uint32_t lanes = (uint32_t)(warp % 4) * 32 << 16;
       const uint32_t ts = tmem + lanes + w * TK, tp = tmem + lanes + C::P0 + w * C::PCOLS, to = tmem + lanes + C::O0 + w * HDP;
-      constexpr float RAISE = SPLIT ? 0.f : 8.f;   // log2 by which a row may outgrow m
-      constexpr float BIAS = SPLIT ? 15.f : 0.f;   // P = 2^BIAS at the maximum
+      constexpr float RAISE = SPLIT ? 4.f : 8.f;   // log2 by which a row may outgrow m
+      constexpr float BIAS = SPLIT ? 11.f : 0.f;   // P = 2^BIAS at m
       float m = -INFINITY, l = 0.f;  // m in scaled log2 units
       bool ok = true;
       auto done = [&](uint64_t* bar) {  // what this warp's lanes did in TMEM so far
@@ -464,7 +473,7 @@ __global__ void __launch_bounds__(TT, 1)
         if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
         fence_after();
         // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
-        const int e0 = n * PPT;
+        const int e0 = (n_first + n) * PPT;
         const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
                            (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
         if (!inner) {
@@ -554,7 +563,25 @@ __global__ void __launch_bounds__(TT, 1)
         ok = wait_warp(&c->pv_done[w], (nk - 1) & 1, c);
         fence_after();
       }
-      if (ok) {
+      if (parts > 1) asm volatile("bar.sync 1, %0;" ::"r"(n_tiles * TM) : "memory");  // both row tiles are through
+      if (ok && parts > 1) {
+        // A part of the keys: O, m and l to shared memory (over q and the ring),
+        // 16-byte chunk i of a row at i ^ (row % 8); the cluster adds the parts below.
+        float* o_row = stage + (w * TM + (warp % 4) * 32 + lane) * HD;
+        if (nk > 0) {
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 32) {
+            float o[32];
+            __syncwarp();
+            tmem_ld32(to + d, o);
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4*>(o_row + (((d + k) / 4) ^ (lane & 7)) * 4) =
+                  make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+        ml[w * TM + (warp % 4) * 32 + lane] = make_float2(m, l);
+      } else if (ok) {
         // Through shared memory (the tile's q, whose products are done), so that a warp writes whole rows: 16-byte
         // chunk i of a row at i ^ (row % 8).
         constexpr int ES = SPLIT ? 4 : 2, CH = HD * ES / 16;  // bytes of an output element, chunks of a row
@@ -632,16 +659,16 @@ __global__ void __launch_bounds__(TT, 1)
       }
       return y;
     };
-    int ahead = rows_from(0), y = past_end, in = 0, slot = 0;
+    int ahead = rows_from(n_first * PPT), y = past_end, in = 0, slot = 0;
     uint32_t use = 0;  // how often the slot was filled before
     bool ok = true;
     for (int n = 0; n < nk && ok; ++n) {
       if (in == 0) {
         y = ahead;
-        ahead = rows_from((n + AHEAD) * PPT);
+        ahead = rows_from((n_first + n + AHEAD) * PPT);
       }
       // rows of the last page past the sequence's end
-      const int n_tail = v && n == nk - 1 ? (sp.page(sp.n - 1) + 1) * PG - kv_end : 0;
+      const int n_tail = v && n_first + n == n_all - 1 ? (sp.page(sp.n - 1) + 1) * PG - kv_end : 0;
       if (use > 0 && !(ok = wait_warp(&c->empty[v][slot], (use - 1) & 1, c))) break;
       uint64_t* bar = n_tail > 0 ? &c->tail : &c->full[v][slot];
       if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
@@ -653,7 +680,7 @@ __global__ void __launch_bounds__(TT, 1)
       __syncwarp();
       if (n_tail > 0) {
         ok = wait_warp(&c->tail, 0, c);
-        const int key0 = (sp.n - 1 - n * PPT) * PG + PG - n_tail;
+        const int key0 = (sp.n - 1 - (n_first + n) * PPT) * PG + PG - n_tail;
         for (int x = lane; x < n_tail * 8 * C::HALVES; x += 32) {
           const int key = key0 + x / 8 % n_tail, half = x / 8 / n_tail;
           *reinterpret_cast<uint4*>(tile + half * (TK * 128) + key * 128 + x % 8 * 16) = make_uint4(0, 0, 0, 0);
@@ -738,6 +765,65 @@ __global__ void __launch_bounds__(TT, 1)
     }
     __syncthreads();
   }
+  if (parts > 1) {
+    // Each CTA adds the parts of its share of the rows, in order, each warp a run of rows; lane = (row, part) for the
+    // statistics.  A wait that ran out anywhere leaves garbage, not a wait here: every CTA comes by.
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    constexpr int E = HD / 32, B = 4;  // rows whose reads are under way at a time
+    if (warp < 8) {
+      const int rpw = p.tile_rows / (8 * parts), row0 = (part * 8 + warp) * rpw;
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (lane < rpw * parts && row0 + lane / parts < n_rows) x = *cl.map_shared_rank(&ml[row0 + lane / parts], lane % parts);
+      float m = x.x;
+      for (int d = 1; d < parts; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      if (m == -INFINITY) m = 0.f;
+      float f = exp2_approx(x.x - m);  // 0 for a part without keys of the row
+      float l = x.y * f;
+      for (int d = 1; d < parts; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+      for (int i0 = 0; i0 < rpw && row0 + i0 < n_rows; i0 += B) {
+        float o[B][E] = {};
+        for (int i = 0; i < parts; ++i) {
+          float v[B][E];
+#pragma unroll
+          for (int j = 0; j < B; ++j) {
+            const int row = row0 + i0 + j;
+            const float* po = cl.map_shared_rank(stage + min(row, n_rows - 1) * HD, i);
+            if constexpr (E == 4) {
+              *reinterpret_cast<float4*>(v[j]) = *reinterpret_cast<const float4*>(po + (lane ^ (row & 7)) * 4);
+            } else {
+#pragma unroll
+              for (int e = 0; e < E; ++e) v[j][e] = po[(((lane * E + e) / 4) ^ (row & 7)) * 4 + (lane * E + e) % 4];
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < B; ++j) {
+            const int from = min(i0 + j, rpw - 1) * parts + i;
+            const float fi = __shfl_sync(0xffffffffu, f, from);
+            if (__shfl_sync(0xffffffffu, x.x, from) == -INFINITY) continue;  // what is there was never written
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[j][e] = fmaf(v[j][e], fi, o[j][e]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+          const int row = row0 + i0 + j;
+          const float lr = __shfl_sync(0xffffffffu, l, min(i0 + j, rpw - 1) * parts);
+          if (i0 + j >= rpw || row >= n_rows) continue;  // the same for the warp
+          const int r = t.row0 + row, tok = r / G, h = hk * G + r % G;
+          const bool sees = t.past + tok >= 0;
+          bool finite = true;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            finite = finite && fabsf(o[j][e]) < INFINITY;
+            store_elem(p.out, ((int64_t)(t.q0 + tok) * p.n_head + h) * HD + lane * E + e, sees ? o[j][e] / lr : 0.f, p.io);
+          }
+          if (__any_sync(0xffffffffu, !finite) && sees && lr < INFINITY) recompute_row<KV, HD>(p, t, hk, r);
+        }
+      }
+    }
+    cl.sync();  // nobody leaves while its shared memory is read
+  }
   if (warp == 9) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -746,7 +832,7 @@ __global__ void __launch_bounds__(TT, 1)
 
 // ---- host -----------------------------------------------------------------------------------
 template <class KV, int HD, bool SPLIT>
-cudaError_t launch_t(WindowAttnParams& p, int kv, cudaStream_t st) {
+cudaError_t launch_t(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
   using C = Cfg<HD, SPLIT>;
   CUtensorMap km, vm;
   const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
@@ -755,33 +841,57 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   e = allow_smem<prefill_tc_kernel<KV, HD, SPLIT>>(C::SMEM);
   if (e != cudaSuccess) return e;
-  const int64_t group = p.n_head / p.n_head_kv;
-  const int64_t tiles = p.n_tok * group / TC_ROWS + p.n_seq;
-  prefill_tc_kernel<KV, HD, SPLIT><<<(unsigned)(tiles * p.n_head_kv), TT, C::SMEM, st>>>(p, km, vm);
-  return cudaGetLastError();
+  // Few row tiles: their keys are split over clusters of 2, 4 or 8, as long as all clusters fit the GPU at a time
+  // (clusters of 8 with one CTA to an SM: 15 of them were seen to fit 148 SMs) and a CTA keeps two key tiles; row
+  // tiles of 128 then, if that still leaves half of the SMs without work.
+  const int64_t rows_all = (int64_t)p.n_tok * (p.n_head / p.n_head_kv);
+  auto jobs = [&](int rt) { return ((rows_all + rt - 1) / rt + p.n_seq - 1) * p.n_head_kv; };
+  int64_t pages = p.max_pages;
+  if (p.window > 0) {
+    const int64_t seen = ((int64_t)p.window + p.n_sink + p.n_tok) / PG + 3;
+    pages = seen < pages ? seen : pages;
+  }
+  p.tile_rows = TC_ROWS;
+  p.key_parts = 1;
+  while (p.key_parts < 8 && pages >= (int64_t)p.key_parts * 4 * C::PPT &&
+         jobs(TC_ROWS) * p.key_parts * 2 <= (p.key_parts == 4 ? sm_count * 8 / 10 : p.key_parts == 2 ? sm_count * 9 / 10 : sm_count))
+    p.key_parts *= 2;
+  if (jobs(TM) * p.key_parts <= sm_count * 8 / 10) p.tile_rows = TM;
+  const int64_t tiles = rows_all / p.tile_rows + p.n_seq;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * p.n_head_kv * p.key_parts));
+  cfg.blockDim = dim3(TT);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)p.key_parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prefill_tc_kernel<KV, HD, SPLIT>, p, km, vm);
 }
 
 template <class KV, bool SPLIT>
-cudaError_t launch_hd(WindowAttnParams& p, int kv, int hd, cudaStream_t st) {
-  if (hd == 32) return launch_t<KV, 32, SPLIT>(p, kv, st);
-  if (hd == 64) return launch_t<KV, 64, SPLIT>(p, kv, st);
-  return launch_t<KV, 128, SPLIT>(p, kv, st);
+cudaError_t launch_hd(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {
+  if (hd == 32) return launch_t<KV, 32, SPLIT>(p, kv, sm_count, st);
+  if (hd == 64) return launch_t<KV, 64, SPLIT>(p, kv, sm_count, st);
+  return launch_t<KV, 128, SPLIT>(p, kv, sm_count, st);
 }
 
 }  // namespace
 
 bool prefill_tc_takes(const WindowAttnParams& p, int kv, int hd) {
   const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
-  const int64_t tiles = (int64_t)p.n_tok * (p.n_head / p.n_head_kv) / TC_ROWS + p.n_seq;
-  if (hd > 128 || rows >= 0x7fffffff || tiles * p.n_head_kv > 0x7fffffff) return false;
+  const int64_t tiles = (int64_t)p.n_tok * (p.n_head / p.n_head_kv) / TM + p.n_seq;
+  if (hd > 128 || rows >= 0x7fffffff || tiles * p.n_head_kv * 8 > 0x7fffffff) return false;
   return kv == EL_F16 || (kv == EL_BF16 && p.io == EL_BF16);
 }
 
 cudaError_t launch_prefill_tc(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {
-  (void)sm_count;
-  if (kv == EL_BF16) return launch_hd<__nv_bfloat16, false>(p, kv, hd, st);
-  if (p.io == EL_F32) return launch_hd<__half, true>(p, kv, hd, st);
-  return launch_hd<__half, false>(p, kv, hd, st);
+  if (kv == EL_BF16) return launch_hd<__nv_bfloat16, false>(p, kv, hd, sm_count, st);
+  if (p.io == EL_F32) return launch_hd<__half, true>(p, kv, hd, sm_count, st);
+  return launch_hd<__half, false>(p, kv, hd, sm_count, st);
 }
 
 }  // namespace sfk

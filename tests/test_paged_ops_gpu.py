@@ -364,7 +364,7 @@ def test_prefill_head_layouts(cuda, io, kv, hq, hkv):
 
 @pytest.mark.parametrize("io,kv,hd", [(F16, F16, 64), (BF16, BF16, 128), (F32, F16, 128)])
 @pytest.mark.parametrize("n_qs,pasts,window,n_sink", [
-    ([1200], [0], 0, 0), ([1200], [0], 256, 4), ([700], [1500], 500, 200), ([5], [3000], 0, 0), ([5], [3000], 100, 16),
+    ([1200], [0], 0, 0), ([1200], [0], 256, 4), ([700], [1500], 500, 200), ([5], [3000], 0, 0), ([5], [3000], 100, 16), ([70], [2500], 0, 0), ([33, 1], [1000, 4000], 900, 3),
     ([1] * 40, list(range(40)), 0, 0), ([600, 600], [0, 640], 64, 0), ([256], [0], 0, 0), ([257], [255], 1000, 1)])
 def test_prefill_lengths(cuda, io, kv, hd, n_qs, pasts, window, n_sink):
     run_prefill(n_qs, pasts, 8, 2, hd, io, kv, window, n_sink, seed=len(n_qs) + window)
@@ -377,18 +377,23 @@ def test_prefill_large_scores(cuda):
     run_prefill([200], [0], 8, 2, 128, F32, F16, 0, 0, scale=1e6, qscale=1e-7)
 
 
+@pytest.mark.parametrize("n_q,past", [(200, 60), (130, 700)])
 @pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 128)])
-def test_prefill_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd):
+def test_prefill_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd, n_q, past):
     """A key whose value is infinite or NaN touches the rows that see it and no other, in the same tile too."""
     from strataflow_b200 import ops
-    q, c, start, kv_len, _ = run_prefill([200], [60], 8, 2, hd, io, kv, 90, 2, gap=0)
-    for j, x in ((150, math.inf), (100, math.nan)):
+    window, n_sink = n_q * 9 // 20, 2
+    q, c, start, kv_len, _ = run_prefill([n_q], [past], 8, 2, hd, io, kv, window, n_sink, gap=0)
+    bad = (past + n_q * 9 // 20, past + n_q // 5)
+    for j, x in zip(bad, (math.inf, math.nan)):
         c.v[c.table[0, j // PG], :, j % PG] = x
-    got = ops.attn_prefill_window(q, c.k, c.v, c.table, start, kv_len, window=90, n_sink=2)
-    p = 60 + torch.arange(200, device="cuda")
-    touched = ((p >= 150) & (p < 240)) | ((p >= 100) & (p < 190))
+    got = ops.attn_prefill_window(q, c.k, c.v, c.table, start, kv_len, window=window, n_sink=n_sink)
+    p = past + torch.arange(n_q, device="cuda")
+    touched = torch.zeros_like(p, dtype=torch.bool)
+    for j in bad:
+        touched |= (p >= j) & (p < j + window)
     assert not torch.isfinite(got[touched]).any()
-    want, tol, absv = reference(q, c.keys[0], c.values[0], range(60, 260), 90, 2)
+    want, tol, absv = reference(q, c.keys[0], c.values[0], range(past, past + n_q), window, n_sink)
     if io != F32:
         tol = tol + half_step(io) * want.abs() + weight_tol(kv, absv)
     check(got.view_as(want)[~touched], want[~touched], tol[~touched])
