@@ -14,7 +14,9 @@
 // S, P and O of both row tiles live in TMEM side by side: S(n + 1) is computed as
 // soon as S(n) is in registers, under the exponentials of S(n), so a softmax warp
 // goes from tile to tile without waiting for the tensor core.  That sets TK: 80 keys
-// at head width 128 (S 2 x 80, P 2 x 40, O 2 x 128 of 512 columns), 128 at 64.
+// at head width 128 (S 2 x 80, P 2 x 40, O 2 x 128 of 512 columns); at 64 there would
+// be room for 128, and 96 were faster (245 and 252 us for a ragged batch of 7308
+// tokens of 32 heads, 123 GFLOP): a row of 128 leaves too few registers.
 // (P over S with 128 keys, the products of a tile in one chain with its softmax, took
 // 892 us for 2048 tokens at 30000 keys, 32 heads of 128.)
 // One thread issues in about 30 cycles a product and 100 a wait: Q K^T and P V
@@ -50,15 +52,13 @@ namespace cg = cooperative_groups;
 constexpr int TM = 128;       // rows per tile
 constexpr int TC_ROWS = 256;  // rows per CTA
 constexpr int TT = 384;       // threads: three warpgroups, 168 registers each at launch
-constexpr int POLY_OF_8 = 2;  // of 8 exponentials, how many go to the multiply-add unit
-
 template <int HD, bool SPLIT>
 struct Cfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;  // head width in shared memory (the copy fills with zeros)
   static constexpr int HALVES = HDP / 64;        // 128-byte column blocks
   static constexpr int NS = SPLIT ? 2 : 1;       // terms of q and P
   // Keys per tile: S (TK columns), P (TK / 2 a term) and O (HDP) of two row tiles share the 512 columns of TMEM
-  static constexpr int TK = HDP == 64 ? (SPLIT ? 96 : 128) : (SPLIT ? 64 : 80);
+  static constexpr int TK = HDP == 64 ? 96 : (SPLIT ? 64 : 80);
   static constexpr int PPT = TK / PG;            // pages per key tile
   static constexpr int TILE = TK * HDP * 2;      // bytes of a K or V tile
   static constexpr int QTILE = TM * HDP * 2;     // bytes of a q term of a row tile
@@ -67,8 +67,11 @@ struct Cfg {
   static constexpr int STAGES = FIT > 4 ? 4 : FIT;  // K tiles, and V tiles, under way
   static constexpr int SMEM = 1024 + QB + 2 * STAGES * TILE + 512;
   static constexpr int FIRST = (PPT + 1) / 2 * PG;  // keys of the first part of P
+  // Of 8 exponentials, how many go to the multiply-add unit (0 / 1 / 2 / 3: 1003 / 946 / 933 / 944 us at width 128,
+  // 2048 tokens at 30000 keys; 1 / 2 / 3: 233 / 238 / 253 at 64, the ragged batch)
+  static constexpr int POLY_OF_8 = SPLIT ? 0 : HDP == 64 ? 1 : 2;
   // Registers after the split: 384 x 168 is what the launch holds.  A softmax thread holds a row of S.
-  static constexpr int REG_SOFTMAX = TK == 128 ? 208 : 184, REG_OTHER = TK == 128 ? 88 : 136;
+  static constexpr int REG_SOFTMAX = 184, REG_OTHER = 136;
   static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
   // TMEM columns
   static constexpr int P0 = 2 * TK, PCOLS = TK / 2 * NS, O0 = 512 - 2 * HDP;
@@ -171,21 +174,6 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[96]) {
       "tcgen05.wait::ld.sync.aligned;"
       : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64)
       : "r"(addr), "r"(addr + 32), "r"(addr + 64)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[128]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,"
-      "%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64), R32("=f", v, 96)
-      : "r"(addr), "r"(addr + 32), "r"(addr + 64), "r"(addr + 96)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
@@ -481,6 +469,7 @@ __global__ void __launch_bounds__(TT, 1)
 #pragma unroll 1
           for (int g = 0; g < PPT; ++g) {
             const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
+            if (jb + PG - 1 <= t_lo && (p.window == 0 || jb > t_hi - p.window)) continue;  // every row sees the page
             const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
             float s[16];
             tmem_ld16(ts + g * PG, s);
@@ -531,7 +520,7 @@ __global__ void __launch_bounds__(TT, 1)
           for (int k = 0; k < 8; ++k) {
             const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, neg2);
             float x, y;
-            if (!SPLIT && (k * 3) % 8 < POLY_OF_8) {
+            if ((k * 3) % 8 < C::POLY_OF_8) {
               exp2_poly<BF16 ? 3 : 4>(x2, x, y);
             } else {
               unpair(x2, x, y);
@@ -842,7 +831,7 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st)
   e = allow_smem<prefill_tc_kernel<KV, HD, SPLIT>>(C::SMEM);
   if (e != cudaSuccess) return e;
   // Few row tiles: their keys are split over clusters of 2, 4 or 8, as long as all clusters fit the GPU at a time
-  // (clusters of 8 with one CTA to an SM: 15 of them were seen to fit 148 SMs) and a CTA keeps two key tiles; row
+  // (clusters of 8 with one CTA to an SM: 15 of them were seen to fit 148 SMs) and a CTA keeps four key tiles; row
   // tiles of 128 then, if that still leaves half of the SMs without work.
   const int64_t rows_all = (int64_t)p.n_tok * (p.n_head / p.n_head_kv);
   auto jobs = [&](int rt) { return ((rows_all + rt - 1) / rt + p.n_seq - 1) * p.n_head_kv; };
@@ -853,7 +842,7 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st)
   }
   p.tile_rows = TC_ROWS;
   p.key_parts = 1;
-  while (p.key_parts < 8 && pages >= (int64_t)p.key_parts * 4 * C::PPT &&
+  while (p.key_parts < 8 && pages >= (int64_t)p.key_parts * 8 * C::PPT &&
          jobs(TC_ROWS) * p.key_parts * 2 <= (p.key_parts == 4 ? sm_count * 8 / 10 : p.key_parts == 2 ? sm_count * 9 / 10 : sm_count))
     p.key_parts *= 2;
   if (jobs(TM) * p.key_parts <= sm_count * 8 / 10) p.tile_rows = TM;
