@@ -50,22 +50,24 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int TM = 128;       // rows per tile
-constexpr int TC_ROWS = 256;  // rows per CTA
 constexpr int TT = 384;       // threads: three warpgroups, 168 registers each at launch
 template <int HD, bool SPLIT>
 struct Cfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;  // head width in shared memory (the copy fills with zeros)
   static constexpr int HALVES = HDP / 64;        // 128-byte column blocks
   static constexpr int NS = SPLIT ? 2 : 1;       // terms of q and P
-  // Keys per tile: S (TK columns), P (TK / 2 a term) and O (HDP) of two row tiles share the 512 columns of TMEM
-  static constexpr int TK = HDP == 64 ? 96 : (SPLIT ? 64 : 80);
+  static constexpr int TILES = SPLIT ? 1 : 2;    // row tiles per CTA
+  static constexpr int ROWS = TILES * TM;
+  // Keys per tile: S (TK columns), P (TK / 2 a term) and O (HDP) of two row tiles, or of one with a second O, share
+  // the 512 columns of TMEM
+  static constexpr int TK = HDP == 64 || SPLIT ? 96 : 80;
   static constexpr int PPT = TK / PG;            // pages per key tile
   static constexpr int TILE = TK * HDP * 2;      // bytes of a K or V tile
   static constexpr int QTILE = TM * HDP * 2;     // bytes of a q term of a row tile
-  static constexpr int QB = 2 * NS * QTILE;
+  static constexpr int QB = TILES * NS * QTILE;
   static constexpr int FIT = (224 * 1024 - QB) / (2 * TILE);
   static constexpr int STAGES = FIT > 4 ? 4 : FIT;  // K tiles, and V tiles, under way
-  static constexpr int SMEM = 1024 + QB + 2 * STAGES * TILE + 512;
+  static constexpr int SMEM = 1024 + QB + 2 * STAGES * TILE + (SPLIT ? 4096 : 512);
   static constexpr int FIRST = (PPT + 1) / 2 * PG;  // keys of the first part of P
   // Of 8 exponentials, how many go to the multiply-add unit (0 / 1 / 2 / 3: 1003 / 946 / 933 / 944 us at width 128,
   // 2048 tokens at 30000 keys; 1 / 2 / 3: 233 / 238 / 253 at 64, the ragged batch)
@@ -74,8 +76,8 @@ struct Cfg {
   static constexpr int REG_SOFTMAX = 184, REG_OTHER = 136;
   static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
   // TMEM columns
-  static constexpr int P0 = 2 * TK, PCOLS = TK / 2 * NS, O0 = 512 - 2 * HDP;
-  static_assert(P0 + 2 * PCOLS <= O0 && STAGES >= 2 && TK % PG == 0, "tile sizes");
+  static constexpr int P0 = TILES * TK, PCOLS = TK / 2 * NS, O0 = 512 - 2 * HDP;
+  static_assert(P0 + TILES * PCOLS <= O0 && STAGES >= 2 && TK % PG == 0, "tile sizes");
 };
 
 struct Ctl {
@@ -85,10 +87,13 @@ struct Ctl {
   uint64_t s_full[2], s_free[2];     // S of a row tile is complete / is in registers
   uint64_t p_full[2][2];             // [row tile][part of the keys]: P is written
   uint64_t pv_done[2];               // O is complete and P is free
+  // SPLIT: O of tile n is complete in buffer n % 2 / has been added; the factor of tile n is in slot n % 4
+  uint64_t o_full[2], o_free[2], f_full[4];
   uint64_t drain;
   uint32_t tmem;
   int abort;
 };
+static_assert(sizeof(Ctl) <= 512, "the control block's place");
 
 // Bounded: false after about a second, or once another warp gave up.  Little code, for the loops that call it.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl* c) {
@@ -321,7 +326,7 @@ __global__ void __launch_bounds__(TT, 1)
   const Tile t = find_tile(p, job / p.n_head_kv, p.tile_rows);
   if (t.seq < 0) return;  // the whole cluster
   const int n_rows = (int)min((int64_t)p.tile_rows, (int64_t)t.n_q * G - t.row0);
-  const int n_tiles = n_rows > TM ? 2 : 1;
+  const int n_tiles = n_rows > TM ? 2 : 1;  // row tiles
   const int p_lo = max(t.past + t.row0 / G, 0), p_hi = t.past + (t.row0 + n_rows - 1) / G;
   SeenPages sp;
   sp.n = sp.sink = sp.first = 0;
@@ -345,7 +350,10 @@ __global__ void __launch_bounds__(TT, 1)
       mbar_init(&c->p_full[i][0], 4);
       mbar_init(&c->p_full[i][1], 4);
       mbar_init(&c->pv_done[i], 1);
+      mbar_init(&c->o_full[i], 1);
+      mbar_init(&c->o_free[i], 4);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&c->f_full[i], 4);
     c->abort = 0;
     fence_mbar_init();
   }
@@ -358,13 +366,16 @@ __global__ void __launch_bounds__(TT, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = c->tmem;
-  float* stage = reinterpret_cast<float*>(base);                // [256][HD]: a part's O
-  float2* ml = reinterpret_cast<float2*>(stage + TC_ROWS * HD);  // [256]: its m and l
+  float* stage = reinterpret_cast<float*>(base);                // [ROWS][HD]: a part's O
+  float2* ml = reinterpret_cast<float2*>(stage + C::ROWS * HD);  // [ROWS]: its m and l
+  float* factor = reinterpret_cast<float*>(c) + 128;            // SPLIT: [4][TM] factors of tiles, then m and l [TM]
+  float2* last = reinterpret_cast<float2*>(factor + 4 * TM);
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFTMAX));
     // ---- softmax: thread = row ----
-    const int w = warp / 4;  // row tile
+    const int w = SPLIT ? 0 : warp / 4;  // row tile
+    const bool adds = SPLIT && warp >= 4;  // the warpgroup that keeps the sum of the tiles' O
     if (w < n_tiles) {
       const int row = w * TM + (warp % 4) * 32 + lane;  // row of the CTA
       const bool live = row < n_rows;
@@ -380,7 +391,7 @@ __global__ void __launch_bounds__(TT, 1)
       // first product).  Into shared memory swizzled: 16-byte chunk i of the row's 128-byte block at i ^ (row % 8).
       constexpr int LR = HD / 8, RI = 32 / LR;  // lanes per row, rows per step
       const int64_t my_q = live ? (int64_t)(t.q0 + tok) * p.q_stride + (int64_t)h * HD : -1;
-      if (nk > 0) {
+      if (nk > 0 && !adds) {
         const int ch = lane % LR;
         auto slot = [&](int lr, int c) {  // row of the tile, chunk of the row
           return qs + w * NS * C::QTILE + lr * 128 + c / 8 * (TM * 128) + ((c % 8) ^ (lr & 7)) * 16;
@@ -450,127 +461,33 @@ __global__ void __launch_bounds__(TT, 1)
       const uint32_t ts = tmem + lanes + w * TK, tp = tmem + lanes + C::P0 + w * C::PCOLS, to = tmem + lanes + C::O0 + w * HDP;
       constexpr float RAISE = SPLIT ? 4.f : 8.f;   // log2 by which a row may outgrow m
       constexpr float BIAS = SPLIT ? 11.f : 0.f;   // P = 2^BIAS at m
-      float m = -INFINITY, l = 0.f;  // m in scaled log2 units
       bool ok = true;
       auto done = [&](uint64_t* bar) {  // what this warp's lanes did in TMEM so far
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
       };
-      for (int n = 0; n < nk; ++n) {
-        if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
-        fence_after();
-        // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
-        const int e0 = (n_first + n) * PPT;
-        const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
-                           (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
-        if (!inner) {
-          // what the row does not see becomes -inf, in place
-#pragma unroll 1
-          for (int g = 0; g < PPT; ++g) {
-            const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
-            if (jb + PG - 1 <= t_lo && (p.window == 0 || jb > t_hi - p.window)) continue;  // every row sees the page
-            const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
-            float s[16];
-            tmem_ld16(ts + g * PG, s);
-#pragma unroll
-            for (int k = 0; k < PG; ++k) s[k] = k <= hi && (k > lo || k < sk) ? s[k] : -INFINITY;
-            tmem_st16(ts + g * PG, s);
-          }
-          tmem_st_wait();
-        }
-        float s[TK];
-        tmem_ld(ts, s);
-        if (n + 1 < nk) done(&c->s_free[w]);  // the next Q K^T may begin
-        float m4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int k = 4; k < TK; k += 4)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
-        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        // O is complete and P may be written again (mostly long since)
-        if (n > 0) {
-          if (!(ok = wait_warp(&c->pv_done[w], (n - 1) & 1, c))) break;
-          fence_after();
-        }
-        mx *= scale;
-        if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
-          const float mn = fmaxf(mx, m);
-          const float f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
-          m = mn;
-          l *= f;
-          if (n > 0) {
-#pragma unroll 1
-            for (int d = 0; d < HDP; d += 16) {
-              float o[16];
-              tmem_ld16(to + d, o);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] *= f;
-              tmem_st16(to + d, o);
-            }
-          }
-        }
-        const float neg = BIAS - (m == -INFINITY ? 0.f : m);
-        const uint64_t scale2 = both(scale), neg2 = both(neg);
-        uint64_t sum2 = 0;
-#pragma unroll
-        for (int b = 0; b < PPT; ++b) {  // 16 keys: 8 columns of P
-          uint32_t hi[8], lo[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, neg2);
-            float x, y;
-            if ((k * 3) % 8 < C::POLY_OF_8) {
-              exp2_poly<BF16 ? 3 : 4>(x2, x, y);
-            } else {
-              unpair(x2, x, y);
-              x = exp2_approx(x);
-              y = exp2_approx(y);
-            }
-            sum2 = add2(sum2, pair(x, y));
-            hi[k] = pack2<BF16>(x, y);
-            if constexpr (SPLIT) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-              lo[k] = pack2<false>(x - f.x, y - f.y);
-            }
-          }
-          tmem_st8(tp + b * 8, hi);
-          if constexpr (SPLIT) tmem_st8(tp + TK / 2 + b * 8, lo);
-          if ((b + 1) * PG == C::FIRST) {  // the product of these keys may begin
-            tmem_st_wait();
-            done(&c->p_full[w][0]);
-          }
-        }
-        float l0, l1;
-        unpair(sum2, l0, l1);
-        l += l0 + l1;
-        tmem_st_wait();
-        done(&c->p_full[w][1]);
-      }
-      // ---- out = O / l ----
-      if (nk > 0 && ok) {
-        ok = wait_warp(&c->pv_done[w], (nk - 1) & 1, c);
-        fence_after();
-      }
-      if (parts > 1) asm volatile("bar.sync 1, %0;" ::"r"(n_tiles * TM) : "memory");  // both row tiles are through
-      if (ok && parts > 1) {
+      // ---- out = O / l, columns(d, o) being 32 columns of O from d on ----
+      auto finish = [&](auto columns, float m, float l) {
+        if (parts > 1) {
         // A part of the keys: O, m and l to shared memory (over q and the ring),
         // 16-byte chunk i of a row at i ^ (row % 8); the cluster adds the parts below.
         float* o_row = stage + (w * TM + (warp % 4) * 32 + lane) * HD;
         if (nk > 0) {
-#pragma unroll 1
+#pragma unroll(SPLIT ? HD / 32 : 1)
           for (int d = 0; d < HD; d += 32) {
             float o[32];
             __syncwarp();
-            tmem_ld32(to + d, o);
+            columns(d, o);
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
               *reinterpret_cast<float4*>(o_row + (((d + k) / 4) ^ (lane & 7)) * 4) =
                   make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
         }
-        ml[w * TM + (warp % 4) * 32 + lane] = make_float2(m, l);
-      } else if (ok) {
+          ml[w * TM + (warp % 4) * 32 + lane] = make_float2(m, l);
+          return;
+        }
         // Through shared memory (the tile's q, whose products are done), so that a warp writes whole rows: 16-byte
         // chunk i of a row at i ^ (row % 8).
         constexpr int ES = SPLIT ? 4 : 2, CH = HD * ES / 16;  // bytes of an output element, chunks of a row
@@ -578,10 +495,10 @@ __global__ void __launch_bounds__(TT, 1)
         uint8_t* rows = qs + w * NS * C::QTILE + wrow % TM * (HD * ES);
         const float inv = 1.0f / l;
         bool finite = true;
-#pragma unroll 1
+#pragma unroll(SPLIT ? HD / 32 : 1)
         for (int d = 0; d < HD; d += 32) {
           float o[32];
-          if (nk > 0) tmem_ld32(to + d, o);
+          if (nk > 0) columns(d, o);
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             finite = finite && fabsf(o[k]) < INFINITY;
@@ -625,6 +542,146 @@ __global__ void __launch_bounds__(TT, 1)
           const int src = __ffs(again) - 1;
           again &= again - 1;
           recompute_row<KV, HD>(p, t, hk, __shfl_sync(0xffffffffu, r, src));
+        }
+      };
+      if (!adds) {
+        float m = -INFINITY, l = 0.f;  // m in scaled log2 units
+        for (int n = 0; n < nk; ++n) {
+          if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
+          fence_after();
+          // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
+          const int e0 = (n_first + n) * PPT;
+          const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
+                             (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
+          if (!inner) {
+            // what the row does not see becomes -inf, in place
+#pragma unroll 1
+            for (int g = 0; g < PPT; ++g) {
+              const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
+              if (jb + PG - 1 <= t_lo && (p.window == 0 || jb > t_hi - p.window)) continue;  // every row sees the page
+              const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
+              float s[16];
+              tmem_ld16(ts + g * PG, s);
+#pragma unroll
+              for (int k = 0; k < PG; ++k) s[k] = k <= hi && (k > lo || k < sk) ? s[k] : -INFINITY;
+              tmem_st16(ts + g * PG, s);
+            }
+            tmem_st_wait();
+          }
+          float s[TK];
+          tmem_ld(ts, s);
+          if (n + 1 < nk) done(&c->s_free[w]);  // the next Q K^T may begin
+          float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < TK; k += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
+          float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          // O is complete and P may be written again (mostly long since)
+          if (n > 0) {
+            if (!(ok = wait_warp(&c->pv_done[w], (n - 1) & 1, c))) break;
+            fence_after();
+          }
+          mx *= scale;
+          float f = 1.f;
+          if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
+            const float mn = fmaxf(mx, m);
+            f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+            m = mn;
+            l *= f;
+            if (!SPLIT && n > 0) {
+#pragma unroll 1
+              for (int d = 0; d < HDP; d += 16) {
+                float o[16];
+                tmem_ld16(to + d, o);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] *= f;
+                tmem_st16(to + d, o);
+              }
+            }
+          }
+          if constexpr (SPLIT) {  // the other warpgroup rescales
+            factor[n % 4 * TM + row] = f;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c->f_full[n % 4]);
+          }
+          const float neg = BIAS - (m == -INFINITY ? 0.f : m);
+          const uint64_t scale2 = both(scale), neg2 = both(neg);
+          uint64_t sum2 = 0;
+#pragma unroll
+          for (int b = 0; b < PPT; ++b) {  // 16 keys: 8 columns of P
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, neg2);
+              float x, y;
+              if ((k * 3) % 8 < C::POLY_OF_8) {
+                exp2_poly<BF16 ? 3 : 4>(x2, x, y);
+              } else {
+                unpair(x2, x, y);
+                x = exp2_approx(x);
+                y = exp2_approx(y);
+              }
+              sum2 = add2(sum2, pair(x, y));
+              hi[k] = pack2<BF16>(x, y);
+              if constexpr (SPLIT) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                lo[k] = pack2<false>(x - f.x, y - f.y);
+              }
+            }
+            tmem_st8(tp + b * 8, hi);
+            if constexpr (SPLIT) tmem_st8(tp + TK / 2 + b * 8, lo);
+            if ((b + 1) * PG == C::FIRST) {  // the product of these keys may begin
+              tmem_st_wait();
+              done(&c->p_full[w][0]);
+            }
+          }
+          float l0, l1;
+          unpair(sum2, l0, l1);
+          l += l0 + l1;
+          tmem_st_wait();
+          done(&c->p_full[w][1]);
+        }
+        if constexpr (SPLIT) {
+          last[row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&c->f_full[nk % 4]);
+        } else {
+          if (nk > 0 && ok) {
+            ok = wait_warp(&c->pv_done[w], (nk - 1) & 1, c);
+            fence_after();
+          }
+          if (parts > 1) asm volatile("bar.sync 1, %0;" ::"r"(n_tiles * TM) : "memory");  // both row tiles are through
+          if (ok) finish([&](int d, float(&o)[32]) { tmem_ld32(to + d, o); }, m, l);
+        }
+      } else if constexpr (SPLIT) {
+        // Each tile's O is a product of its own, added here: the tensor core's f32 accumulator drops what falls below
+        // its last bit, a loss that grows with the products on one accumulator (-7.6e-6 of the result over 440 of them).
+        float acc[HD];
+#pragma unroll
+        for (int k = 0; k < HD; ++k) acc[k] = 0.f;
+        for (int n = 0; n < nk; ++n) {
+          if (!(ok = wait_warp(&c->f_full[n % 4], n / 4 & 1, c))) break;
+          const float f = factor[n % 4 * TM + row];
+          if (!(ok = wait_warp(&c->o_full[n % 2], n / 2 & 1, c))) break;
+          fence_after();
+#pragma unroll
+          for (int d = 0; d < HD; d += 32) {
+            float o[32];
+            tmem_ld32(to + n % 2 * HDP + d, o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[d + k] = fmaf(acc[d + k], f, o[k]);
+          }
+          done(&c->o_free[n % 2]);
+        }
+        if (ok && (ok = wait_warp(&c->f_full[nk % 4], nk / 4 & 1, c))) {
+          const float2 x = last[row];
+          finish(
+              [&](int d, float(&o)[32]) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = acc[d + k];
+              },
+              x.x, x.y);
         }
       }
     }
@@ -698,11 +755,11 @@ __global__ void __launch_bounds__(TT, 1)
           fence_after();
           const uint32_t a = q_lo + w * (NS * C::QTILE >> 4), b = k_lo + slot * (C::TILE >> 4), d = tmem + w * TK;
 #pragma unroll
-          for (int s = 0; s < NS; ++s)
+          for (int s = NS - 1; s >= 0; --s)
 #pragma unroll
             for (int k = 0; k < HDP / 16; ++k)
               mma_ss(d, a + ((s * C::QTILE + k / 4 * (TM * 128) + k % 4 * 32) >> 4),
-                     b + ((k / 4 * (TK * 128) + k % 4 * 32) >> 4), QK, s + k > 0);
+                     b + ((k / 4 * (TK * 128) + k % 4 * 32) >> 4), QK, NS - 1 - s + k > 0);
           commit(&c->s_full[w]);
           if (w == n_tiles - 1) commit(&c->empty[0][slot]);
         }
@@ -718,19 +775,24 @@ __global__ void __launch_bounds__(TT, 1)
         if (!(ok = wait(&c->full[1][slot], use & 1, c))) break;
 #pragma unroll 1
         for (int w = 0; w < n_tiles; ++w) {
-          const uint32_t a = tmem + C::P0 + w * C::PCOLS, b = v_lo + slot * (C::TILE >> 4), d = tmem + C::O0 + w * HDP;
+          const uint32_t a = tmem + C::P0 + w * C::PCOLS, b = v_lo + slot * (C::TILE >> 4);
+          const uint32_t d = tmem + C::O0 + (SPLIT ? n % 2 : w) * HDP;
+          if (SPLIT && n > 1 && !(ok = wait(&c->o_free[n % 2], (n / 2 - 1) & 1, c))) break;
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
             if (!(ok = wait(&c->p_full[w][part], n & 1, c))) break;
             fence_after();
+            // the small terms first: they lose nothing to a large sum
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
+            for (int s = NS - 1; s >= 0; --s)
 #pragma unroll
               for (int k = part ? C::FIRST / 16 : 0; k < (part ? TK : C::FIRST) / 16; ++k)
-                mma_ts(d, a + s * (TK / 2) + k * 8, b + (k * 2048 >> 4), PV, part + s + k > 0 ? 1 : n > 0);
+                mma_ts(d, a + s * (TK / 2) + k * 8, b + (k * 2048 >> 4), PV,
+                       part + (NS - 1 - s) + k > 0 ? 1 : !SPLIT && n > 0);
           }
           if (!ok) break;
           commit(&c->pv_done[w]);
+          if (SPLIT) commit(&c->o_full[n % 2]);
           if (w == n_tiles - 1) commit(&c->empty[1][slot]);
         }
         if (++slot == C::STAGES) slot = 0, ++use;
@@ -840,12 +902,12 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st)
     const int64_t seen = ((int64_t)p.window + p.n_sink + p.n_tok) / PG + 3;
     pages = seen < pages ? seen : pages;
   }
-  p.tile_rows = TC_ROWS;
+  p.tile_rows = C::ROWS;
   p.key_parts = 1;
   while (p.key_parts < 8 && pages >= (int64_t)p.key_parts * 8 * C::PPT &&
-         jobs(TC_ROWS) * p.key_parts * 2 <= (p.key_parts == 4 ? sm_count * 8 / 10 : p.key_parts == 2 ? sm_count * 9 / 10 : sm_count))
+         jobs(C::ROWS) * p.key_parts * 2 <= (p.key_parts == 4 ? sm_count * 8 / 10 : p.key_parts == 2 ? sm_count * 9 / 10 : sm_count))
     p.key_parts *= 2;
-  if (jobs(TM) * p.key_parts <= sm_count * 8 / 10) p.tile_rows = TM;
+  if (C::ROWS > TM && jobs(TM) * p.key_parts <= sm_count * 8 / 10) p.tile_rows = TM;
   const int64_t tiles = rows_all / p.tile_rows + p.n_seq;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * p.n_head_kv * p.key_parts));
