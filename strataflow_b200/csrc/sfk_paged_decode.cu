@@ -218,26 +218,87 @@ __device__ __forceinline__ int page_id(const WindowAttnParams& p, const Work& w,
 }
 
 // ---- CUDA cores: any cache type -----------------------------------------------------
-// A warp takes a page at a time.  Scores: lane (g, t) = (lane / 4, lane % 4)
-// multiplies dims 8 t .. 8 t + 7 of each 32 of keys g and g + 8 by the query
-// rows in shared memory.  Values: the lane owns HD / 32 output dims.
+// A warp takes a page at a time.  K and V of a page and head are contiguous: each
+// arrives by one bulk copy in a ring of slots that the warp has to itself (K, V, K,
+// V, ...).  Scores: lane (g, t) multiplies four dims of every 16 of keys g and g + 8
+// by the query rows in shared memory; odd g take the two halves of 32 dims in the
+// other order, so that two keys' rows never meet in a bank.  Values: the lane owns
+// HD / 32 output dims.  64 multiply-adds to 10 shared loads, and 64 bytes of cache a
+// cycle at the multiply-add rate, above what memory delivers.
+template <class KV, int HD>
+struct CcCfg {
+  static constexpr int R = 8, DW = 4;
+  static constexpr int UNIT = PG * HD * (int)sizeof(KV);  // bytes of a page's K or V
+  static constexpr int SLOTS = UNIT <= 4096 ? 6 : 3;
+};
 template <class KV, int HD>
 struct CcSmem {
-  static constexpr int R = 8, DW = 4;
-  float q[R][HD];
-  float p[DW][R][PG];
-  JoinSmem<R, HD, DW> join;
+  using C = CcCfg<KV, HD>;
+  union {
+    uint8_t ring[C::DW][C::SLOTS][C::UNIT];
+    JoinSmem<C::R, HD, C::DW> join;
+  };
+  float q[C::R][HD];
+  float p[C::DW][C::R][PG];
+  uint64_t full[C::DW][C::SLOTS];
 };
+template <class KV>
+__device__ __forceinline__ float4 lds4(const KV* p) {
+  if constexpr (sizeof(KV) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    if constexpr (std::is_same<KV, __nv_bfloat16>::value)
+      return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                         __uint_as_float(w.y & 0xffff0000u));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
 
 template <class KV, int HD>
-__global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(const __grid_constant__ WindowAttnParams p) {
+__global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const __grid_constant__ WindowAttnParams p) {
+  using C = CcCfg<KV, HD>;
   using Smem = CcSmem<KV, HD>;
-  constexpr int R = Smem::R, E = HD / 32, DW = Smem::DW, DT = DW * 32;
+  constexpr int R = C::R, E = HD / 32, DW = C::DW, DT = DW * 32, S = C::SLOTS;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   if (p.partial) pdl_launch_dependents();
   const Work w = find_work<R>(p);
+  const int mine = (w.i1 - w.i0 - warp + DW - 1) / DW;  // pages of this warp (<= 0: none)
+  if (lane == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&sm.full[warp][i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  // ids of this warp's entries i0 + warp + DW k, k = ids_at .. ids_at + 31; -1: outside the pool
+  int ids = -1, ids_at = -32;
+  unsigned bad = 0;  // bit k % 8: page k is outside the pool
+  auto issue = [&](int j) {  // unit j: K (even) or V (odd) of page j / 2
+    const int k = j / 2;
+    if (k >= mine) return;
+    if (k - ids_at >= 32) {
+      const int i = w.i0 + warp + DW * (k + lane);
+      ids = i < w.i1 ? page_id(p, w, i) : -1;
+      ids_at = k;
+    }
+    const int id = __shfl_sync(0xffffffffu, ids, k - ids_at);
+    bad = id < 0 ? bad | 1u << (k % 8) : bad & ~(1u << (k % 8));
+    if (lane == 0) {
+      uint64_t* bar = &sm.full[warp][j % S];
+      if (id < 0) {
+        mbar_arrive(bar);
+      } else {
+        mbar_arrive_expect_tx(bar, C::UNIT);
+        bulk_g2s(sm.ring[warp][j % S],
+                 static_cast<const KV*>(j & 1 ? p.v_pages : p.k_pages) + ((int64_t)id * p.n_head_kv + w.hk) * PG * HD,
+                 C::UNIT, bar);
+      }
+    }
+  };
+  for (int j = 0; j < S; ++j) issue(j);
   for (int i = tid; i < R * HD; i += DT) {
     const int r = i / HD;
     sm.q[r][i % HD] = r < w.n_rows ? load_elem(p.q, w.seq * p.q_stride + (int64_t)(w.head0 + r) * HD + i % HD, p.io) : 0.f;
@@ -251,37 +312,29 @@ __global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(cons
 #pragma unroll
     for (int e = 0; e < E; ++e) o[r][e] = 0.f;
   }
-  for (int i = w.i0 + warp; i < w.i1; i += DW) {
-    const int id = page_id(p, w, i);
-    if (id < 0) continue;
-    const int64_t off = ((int64_t)id * p.n_head_kv + w.hk) * PG * HD;
-    const KV* kp = static_cast<const KV*>(p.k_pages) + off;
-    const KV* vp = static_cast<const KV*>(p.v_pages) + off;
-    const int j0 = w.sp.page(i) * PG;
+  for (int k = 0; k < mine; ++k) {
+    const int j0 = w.sp.page(w.i0 + warp + DW * k) * PG;
+    const bool gone = bad >> (k % 8) & 1;
+    bool ok = wait_slot(&sm.full[warp][2 * k % S], (uint32_t)(2 * k / S) & 1, p.status);
+    const KV* kp = reinterpret_cast<const KV*>(sm.ring[warp][2 * k % S]) + g * HD + t * 4;
     float s[R][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = 0.f;
-#pragma unroll
-    for (int c = 0; c < HD / 32; ++c) {
-      Raw8<KV> ra, rb;
-      load8(ra, kp + g * HD + c * 32 + t * 8, true);
-      load8(rb, kp + (g + 8) * HD + c * 32 + t * 8, true);
-      float a[8], b[8];
-      unpack8(ra, a);
-      unpack8(rb, b);
+#pragma unroll 2
+    for (int c = 0; c < HD / 16; ++c) {
+      const int d = (c ^ (g & 1)) * 16;
+      const float4 a = lds4<KV>(kp + d), b = lds4<KV>(kp + 8 * HD + d);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        float q[8];
-        *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(&sm.q[r][c * 32 + t * 8]);
-        *reinterpret_cast<float4*>(q + 4) = *reinterpret_cast<const float4*>(&sm.q[r][c * 32 + t * 8 + 4]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          s[r][0] = fmaf(q[e], a[e], s[r][0]);
-          s[r][1] = fmaf(q[e], b[e], s[r][1]);
-        }
+        const float4 q = *reinterpret_cast<const float4*>(&sm.q[r][d + t * 4]);
+        s[r][0] = fmaf(q.x, a.x, fmaf(q.y, a.y, fmaf(q.z, a.z, fmaf(q.w, a.w, s[r][0]))));
+        s[r][1] = fmaf(q.x, b.x, fmaf(q.y, b.y, fmaf(q.z, b.z, fmaf(q.w, b.w, s[r][1]))));
       }
     }
-    const bool see0 = key_seen(j0 + g, w.pos, p.window, p.n_sink), see1 = key_seen(j0 + g + 8, w.pos, p.window, p.n_sink);
+    __syncwarp();
+    issue(2 * k + S);
+    const bool see0 = !gone && key_seen(j0 + g, w.pos, p.window, p.n_sink);
+    const bool see1 = !gone && key_seen(j0 + g + 8, w.pos, p.window, p.n_sink);
     float f[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -293,6 +346,7 @@ __global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(cons
       s[r][0] = see0 ? s[r][0] * p.scale_log2 : -INFINITY;
       s[r][1] = see1 ? s[r][1] * p.scale_log2 : -INFINITY;
       float mx = fmaxf(s[r][0], s[r][1]);
+#pragma unroll
       for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
       mx = fmaxf(mx, m[r]);
       const float ms = mx == -INFINITY ? 0.f : mx;
@@ -310,19 +364,48 @@ __global__ void __launch_bounds__(CcSmem<KV, HD>::DW * 32) decode_cc_kernel(cons
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int e = 0; e < E; ++e) o[r][e] *= f[r];
-#pragma unroll 4
-    for (int j = 0; j < PG; ++j) {
-      if (!key_seen(j0 + j, w.pos, p.window, p.n_sink)) continue;  // what a masked place holds is never used
-      float v[E];
+    ok = ok && wait_slot(&sm.full[warp][(2 * k + 1) % S], (uint32_t)((2 * k + 1) / S) & 1, p.status);
+    if (!ok) {
+      const long long t0 = clock64();  // the copies still under way end before their memory is used again
+      while (clock64() - t0 < 1 << 20) {
+      }
+      break;
+    }
+    const KV* vp = reinterpret_cast<const KV*>(sm.ring[warp][(2 * k + 1) % S]) + lane * E;
+    const bool edge = gone || j0 + PG - 1 > w.pos || (p.window > 0 && j0 <= w.pos - p.window);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = to_f32<KV>(vp[j * HD + lane * E + e]);
+    for (int j = 0; j < PG; j += 4) {
+      float v[4][E];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int i = 0; i < 4; ++i) {
+        // what a masked place holds is never used
+        const bool see = !edge || (!gone && key_seen(j0 + j + i, w.pos, p.window, p.n_sink));
+        if constexpr (E % 4 == 0) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[r][e] = fmaf(sm.p[warp][r][j], v[e], o[r][e]);
+          for (int e = 0; e < E; e += 4) {
+            const float4 x = lds4<KV>(vp + (j + i) * HD + e);
+            v[i][e] = see ? x.x : 0.f;
+            v[i][e + 1] = see ? x.y : 0.f;
+            v[i][e + 2] = see ? x.z : 0.f;
+            v[i][e + 3] = see ? x.w : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[i][e] = see ? to_f32<KV>(vp[(j + i) * HD + e]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float4 x = *reinterpret_cast<const float4*>(&sm.p[warp][r][j]);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          o[r][e] = fmaf(x.w, v[3][e], fmaf(x.z, v[2][e], fmaf(x.y, v[1][e], fmaf(x.x, v[0][e], o[r][e]))));
+      }
     }
     __syncwarp();
+    issue(2 * k + 1 + S);
   }
+  __syncthreads();  // the ring becomes the join's memory
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     for (int d = 4; d < 32; d *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
@@ -689,8 +772,9 @@ void pick_parts(WindowAttnParams& p, int occ, int hd, int sm_count) {
 template <class KV, int HD>
 cudaError_t launch_cc(WindowAttnParams& p, int sm_count, cudaStream_t st) {
   using Smem = CcSmem<KV, HD>;
-  static_assert(Smem::R == DEC_R && Smem::DW == DEC_W, "pick_parts counts these");
-  pick_parts(p, 2, HD, sm_count);
+  using C = CcCfg<KV, HD>;
+  static_assert(C::R == DEC_R && C::DW == DEC_W, "pick_parts counts these");
+  pick_parts(p, sizeof(Smem) > 113 * 1024 ? 1 : 2, HD, sm_count);
   return launch_parts<decode_cc_kernel<KV, HD>>(p, row_tiles(p), DEC_W * 32, sizeof(Smem), st);
 }
 
