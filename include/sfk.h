@@ -518,6 +518,8 @@ SFK_API sfk_status sfk_attn_decode_paged(const float *dev_q, const void *dev_k_p
  *     position, length, sequence or page id outside its range is never
  *     dereferenced; it stores a code there, and sfk_device_status (which waits
  *     for the stream) turns the code into SFK_ERR_RUNTIME and clears the word.
+ *     What the call then gives for that sequence is not specified; the others
+ *     are not touched by it.
  */
 
 /* q, k (optionally) normed and rotated, q to q_out, k and v appended to the
@@ -567,7 +569,7 @@ SFK_API sfk_status sfk_attn_decode_window(int32_t io_type, const void *dev_q, in
 SFK_API size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
                                                 int32_t max_pages, int32_t window, int32_t n_sink);
 
-/* The same attention for the newest tokens of each of n_seq sequences: rows
+/* The same attention for the newest tokens of each of n_seq <= 65535 sequences: rows
  * q_start[s] .. q_start[s+1]-1 of q (q_start [n_seq + 1], ascending, device)
  * are the last n_q of the kv_len[s] tokens that sequence s has in the cache
  * (kv_len device), and token i of them sits at position kv_len[s] - n_q + i.

@@ -261,26 +261,32 @@ struct Tile {
   int past;                // position of its first token
 };
 __device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx, int RT) {
+  constexpr int V = 4;  // sequences of a lane: one round trip to memory for 128 of them
   const int lane = threadIdx.x & 31;
   const int64_t group = p.n_head / p.n_head_kv;
   Tile t;
   t.seq = -1;
-  for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
-    const int s = s0 + lane;
-    int a = 0, n = 0, len = 0;
-    int64_t tiles = 0;
-    if (s < p.n_seq) {
-      a = p.q_start[s];
-      const int b = p.q_start[s + 1];
-      len = p.kv_len[s];
-      if (a < 0 || b < a || b > p.n_tok || len < 0 || (len + PG - 1) / PG > p.max_pages) {
-        report(p.status, ERR_BAD_POS);  // nothing of this sequence is read or written
-      } else {
-        n = b - a;
-        tiles = (n * group + RT - 1) / RT;
+  for (int s0 = 0; s0 < p.n_seq; s0 += 32 * V) {
+    const int s = s0 + lane * V;
+    int at[V + 1], len[V], n[V];
+    int64_t tiles[V], sum = 0;
+#pragma unroll
+    for (int i = 0; i <= V; ++i) at[i] = s + i <= p.n_seq ? p.q_start[s + i] : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) len[i] = s + i < p.n_seq ? p.kv_len[s + i] : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      n[i] = 0;
+      if (s + i < p.n_seq) {
+        if (at[i] < 0 || at[i + 1] < at[i] || at[i + 1] > p.n_tok || len[i] < 0 || (len[i] + (int64_t)PG - 1) / PG > p.max_pages)
+          report(p.status, ERR_BAD_POS);  // nothing of this sequence is read or written
+        else
+          n[i] = at[i + 1] - at[i];
       }
+      tiles[i] = (n[i] * group + RT - 1) / RT;
+      sum += tiles[i];
     }
-    int64_t incl = tiles;
+    int64_t incl = sum;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
@@ -289,13 +295,27 @@ __device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx
     const unsigned hit = __ballot_sync(0xffffffffu, idx < incl);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int64_t before = __shfl_sync(0xffffffffu, incl - tiles, src);
-      const int64_t cnt = __shfl_sync(0xffffffffu, tiles, src);
-      t.seq = s0 + src;
-      t.q0 = __shfl_sync(0xffffffffu, a, src);
-      t.n_q = __shfl_sync(0xffffffffu, n, src);
-      t.past = __shfl_sync(0xffffffffu, len, src) - t.n_q;
-      t.row0 = (int)((cnt - 1 - (idx - before)) * RT);
+      // the lane that holds it picks the sequence
+      int64_t left = idx - (incl - sum), cnt = 0;
+      int seq = 0, q0 = 0, nq = 0, kv = 0;
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!found && left < tiles[i]) {
+          found = true;
+          seq = s + i;
+          q0 = at[i];
+          nq = n[i];
+          kv = len[i];
+          cnt = tiles[i];
+        }
+        if (!found) left -= tiles[i];
+      }
+      t.seq = __shfl_sync(0xffffffffu, seq, src);
+      t.q0 = __shfl_sync(0xffffffffu, q0, src);
+      t.n_q = __shfl_sync(0xffffffffu, nq, src);
+      t.past = __shfl_sync(0xffffffffu, kv, src) - t.n_q;
+      t.row0 = (int)((__shfl_sync(0xffffffffu, cnt, src) - 1 - __shfl_sync(0xffffffffu, left, src)) * RT);
       return t;
     }
     idx -= __shfl_sync(0xffffffffu, incl, 31);

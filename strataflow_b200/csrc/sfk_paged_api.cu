@@ -199,7 +199,7 @@ sfk_status sfk_attn_prefill_window(int32_t io_type, const void* q, int64_t q_str
                                    int32_t n_head, int32_t n_head_kv, int32_t hd, float scale, int32_t window,
                                    int32_t n_sink, void* out, int32_t* status, void* stream) {
   const char* who = "attn_prefill_window";
-  if (n_seq < 0 || n_tok < 0) BAD("%s: sizes (%d tokens, %d sequences)", who, n_tok, n_seq);
+  if (n_seq < 0 || n_tok < 0 || n_seq > 65535) BAD("%s: sizes (%d tokens, %d sequences)", who, n_tok, n_seq);
   if (n_seq == 0 || n_tok == 0) return SFK_OK;
   WindowAttnParams a{};
   int kv = 0;

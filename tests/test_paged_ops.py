@@ -70,7 +70,7 @@ def test_decode_refusals(sfk, kw, why):
 
 
 @pytest.mark.parametrize("kw,why", ATTN + [(dict(start=None), b"null"), (dict(lens=None), b"null"), (dict(n=-1), b"sizes"),
-                                           (dict(n_tok=-1), b"sizes"), (dict(n_tok=1 << 29), b"in one call")])
+                                           (dict(n_tok=-1), b"sizes"), (dict(n=65536), b"sizes"), (dict(n_tok=1 << 29), b"in one call")])
 def test_prefill_refusals(sfk, kw, why):
     assert call(sfk, "sfk_attn_prefill_window", PREFILL, **kw) == L.SFK_ERR_INVALID_ARGUMENT
     assert why in sfk.sfk_last_error()

@@ -268,6 +268,35 @@ def test_decode_batches_and_lengths(cuda, io, kv, lens):
     run_decode(lens, 8, 2, 128, io, kv, 0, 0, seed=len(lens))
 
 
+@pytest.mark.parametrize("io,kv", [(F32, F16), (BF16, BF16), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_decode_long_windows(cuda, io, kv, hd):
+    """Windows long enough to be split over many CTAs, a start inside a page, more sinks than a page holds."""
+    run_decode([20000, 300, 9001], 4, 1, hd, io, kv, 9000, 40, seed=hd)
+
+
+def test_decode_with_a_wide_table(cuda):
+    """A table for far longer contexts than the sequences have; without a workspace the result is the same."""
+    from strataflow_b200 import lib as L
+    from strataflow_b200 import ops
+    c = Cache([700, 40, 0], 2, 128, BF16, 1)
+    table = torch.full((3, 5000), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    q = torch.randn((3, 8, 128), generator=gen(2), device="cuda").to(BF16)
+    pos = torch.tensor([699, 39, -1], dtype=torch.int32, device="cuda")
+    got = ops.attn_decode_window(q, c.k, c.v, table, pos)
+    bare = torch.empty_like(got)
+    L.check(L.load().sfk_attn_decode_window(L.TYPE_BF16, q.data_ptr(), 8 * 128, L.KV_BF16, c.k.data_ptr(), c.v.data_ptr(),
+                                            c.k.shape[0], table.data_ptr(), 5000, pos.data_ptr(), 3, 8, 2, 128, 0.0, 0, 0,
+                                            bare.data_ptr(), None, 0, None, torch.cuda.current_stream().cuda_stream))
+    for s, n in enumerate((700, 40)):
+        want, tol, _ = reference(q[s:s + 1], c.keys[s], c.values[s], [n - 1], 0, 0)
+        tol = tol + half_step(BF16) * want.abs()
+        check(got[s:s + 1].view_as(want), want, tol)
+        check(bare[s:s + 1].view_as(want), want, tol)
+    assert (got[2] == 0).all() and (bare[2] == 0).all()
+
+
 def test_decode_large_scores(cuda):
     """Scores in the hundreds: the running maximum decides; f16 keys and 32-bit queries far from 1."""
     run_decode([700], 8, 2, 128, F32, F16, 0, 0, scale=1.0, qscale=30.0)
@@ -368,6 +397,31 @@ def test_prefill_head_layouts(cuda, io, kv, hq, hkv):
     ([1] * 40, list(range(40)), 0, 0), ([600, 600], [0, 640], 64, 0), ([256], [0], 0, 0), ([257], [255], 1000, 1)])
 def test_prefill_lengths(cuda, io, kv, hd, n_qs, pasts, window, n_sink):
     run_prefill(n_qs, pasts, 8, 2, hd, io, kv, window, n_sink, seed=len(n_qs) + window)
+
+
+@pytest.mark.parametrize("io,kv,hd", [(BF16, BF16, 128), (F32, F16, 64), (F32, F32, 32)])
+def test_prefill_many_sequences(cuda, io, kv, hd):
+    """More sequences than one look at the batch takes, most of them with one token or none."""
+    n_qs = [(i * 7) % 5 if i % 3 else 1 for i in range(300)]
+    run_prefill(n_qs, [(i * 37) % 90 for i in range(300)], 4, 2, hd, io, kv, 20, 1)
+
+
+def test_prefill_long_context_keeps_32_bits(cuda):
+    """32-bit rows at 30000 keys: within the bound, and free of the drift that one accumulator over all keys shows."""
+    from strataflow_b200 import ops
+    for n_q, past in ((300, 30000), (3, 30000)):
+        c = Cache([n_q + past], 1, 128, F16, 5)
+        q = torch.randn((n_q, 4, 128), generator=gen(6), device="cuda")
+        start = torch.tensor([0, n_q], dtype=torch.int32, device="cuda")
+        got = ops.attn_prefill_window(q, c.k, c.v, c.table, start, start[1:] + past).view_as(q)
+        want = torch.cat([reference(q[i:i + 30], c.keys[0], c.values[0], range(past + i, past + min(i + 30, n_q)), 0, 0)[0]
+                          for i in range(0, n_q, 30)])
+        # The accumulator truncates: a loss of 2^-24 of the sum on average each time.  A tile is 12 of them: a gain
+        # 12 * 2^-24 = 7.2e-7 below 1 at most, where one accumulator over all keys (3800 of them) would lose 2e-4 at
+        # most and lost 7.6e-6 over 440.  Beside it: 8 truncations of a score (rms 1.5: 8 * 2^-24 * 1.5 = 7.2e-7), the
+        # exponential and the two terms of P (2^-22 each): 1.1e-6 as a root of squares, below 2^-19.
+        assert abs(float((got * want).sum() / (want * want).sum()) - 1) < 2.0 ** -20
+        assert float((got - want).norm() / want.norm()) < 2.0 ** -19
 
 
 def test_prefill_large_scores(cuda):
