@@ -437,6 +437,12 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 // halves of S and of O are added.  P reaches 2^BIAS, so that its second term keeps
 // clear of f16's smallest step; the running maximum moves when a row outgrows it by
 // 2^RAISE.
+// Eight sequences of 131072 keys, 64 heads of 128 over 8, bf16: 645 us, 6.66 TB/s, what a
+// copy reaches (operands straight from global memory: 1190 us).  One sequence of
+// 32768, f32 rows over f16: 29.8 us, of which 20.5 are the bytes and the rest the chain
+// before the first page and behind the last one.  Three CTAs of two slots a warp,
+// not two of three: 38 and 49 us for 48 ragged windows of 1024, 645 and 647 for the
+// eight long ones.
 constexpr int MMA_R = 8;
 
 template <bool BF16>
@@ -743,7 +749,8 @@ int row_tiles(const WindowAttnParams& p) { return (p.n_head / p.n_head_kv + DEC_
 // Short contexts: a cluster of up to 8, doubled until the GPU has two CTAs for
 // every SM, as long as each warp keeps a page or more.  Where a warp would still
 // walk more than LONG pages that way, the pages are split into one wave of `occ`
-// CTAs per SM, joined through the workspace.
+// CTAs per SM, joined through the workspace (one sequence, 8 kv heads: 12.4 us in clusters and
+// 8.8 split at 4096 keys; 6.3 and 7.5 at 1024).
 constexpr int LONG = 2;
 struct Parts {
   int cluster;    // CTAs per cluster without a workspace
