@@ -191,15 +191,13 @@ def _cuda_device(t: torch.Tensor, what: str) -> int:
     return dev
 
 
-def _call(dev: int, fn, *args) -> None:
-    """Run an entry on device `dev`'s current stream (the library launches on the current device)."""
-    if dev == torch.cuda.current_device():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if status:
-        L.check(status)
+def _elsewhere(dev: int) -> bool:
+    """Whether `dev` is not the current device, on which the library launches."""
+    return dev != torch.cuda.current_device()
+
+
+def _stream_of(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _status(status: torch.Tensor | None, dev: int) -> int | None:
@@ -210,7 +208,8 @@ def check_status(status: torch.Tensor) -> None:
     """Wait for the current stream; raise SfkError if the status word of earlier
     paged-cache calls records an error, and clear it."""
     dev = _cuda_device(status, "status")
-    _call(dev, L.load().sfk_device_status, _status(status, dev))
+    with torch.cuda.device(dev):
+        L.check(L.load().sfk_device_status(_status(status, dev), _stream_of(dev)))
 
 
 def rope_freqs(n_rot: int, base: float = 10000.0, scale: float = 1.0, device="cuda") -> torch.Tensor:
@@ -246,35 +245,49 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     q).  rope_pos [n_axes][tokens] with axes (rope_axes) replaces the cache
     positions in the rotation.  Rows with pos < 0 are padding."""
     dev = _cuda_device(q, "q")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return qk_norm_rope_append(q, k, v, k_pages, v_pages, page_table, pos, seq=seq, freqs=freqs, neox=neox,
+                                       q_norm=q_norm, k_norm=k_norm, eps=eps, rope_pos=rope_pos, axes=axes, out=out,
+                                       status=status)
     kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
-    n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-    if q.dtype not in _ROW_TYPES:
-        _refuse(f"q: f32, f16 or bf16 is wanted, got {q.dtype}")
-    qp, qs = _rows(q, "q", heads, hd, q.dtype, dev)
-    kp, ks = _rows(k, "k", kvh, hd, q.dtype, dev)
-    vp, vs = _rows(v, "v", kvh, hd, q.dtype, dev)
+    dtype, shape = q.dtype, q.shape
+    n, heads = shape[0], shape[1] if len(shape) == 3 else 0
+    io = _ROW_TYPES.get(dtype)
+    if io is None:
+        _refuse(f"q: f32, f16 or bf16 is wanted, got {dtype}")
+    qp, qs = _rows(q, "q", heads, hd, dtype, dev)
+    kp, ks = _rows(k, "k", kvh, hd, dtype, dev)
+    vp, vs = _rows(v, "v", kvh, hd, dtype, dev)
     if k.shape[0] != n or v.shape[0] != n:
         _refuse(f"q, k and v: {n}, {k.shape[0]} and {v.shape[0]} tokens")
     if out is None:
-        out = q.new_empty((n, heads, hd))
-    op, os_ = _rows(out, "out", heads, hd, q.dtype, dev)
-    if out.shape[0] != n:
-        _refuse(f"out: {n} tokens are wanted, got {out.shape[0]}")
-    n_rot = 0 if freqs is None else 2 * freqs.numel()
-    n_axes = 0
+        out = q.new_empty(shape)
+        op, os_ = out.data_ptr(), heads * hd
+    else:
+        op, os_ = _rows(out, "out", heads, hd, dtype, dev)
+        if out.shape[0] != n:
+            _refuse(f"out: {n} tokens are wanted, got {out.shape[0]}")
+    n_seq, max_pages = page_table.shape
+    fp, n_rot = None, 0
+    if freqs is not None:
+        n_rot = 2 * freqs.numel()
+        fp = _plain(freqs, "freqs", torch.float32, (n_rot // 2,), dev)
+    rp, n_axes = None, 0
     if rope_pos is not None:
         n_axes = rope_pos.shape[0] if rope_pos.dim() == 2 else 0
-        _int32(rope_pos, "rope_pos", (n_axes, n), dev)
+        rp = _int32(rope_pos, "rope_pos", (n_axes, n), dev)
     if axes is not None and len(axes) != n_rot // 2:
         _refuse(f"axes: {n_rot // 2} pairs are rotated, got {len(axes)}")
-    n_seq = page_table.shape[0]
-    _call(dev, L.load().sfk_qk_norm_rope_append, _ROW_TYPES[q.dtype], qp, qs, kp, ks, vp, vs, n, heads, kvh, hd,
-          _f32(q_norm, "q_norm", hd, dev), _f32(k_norm, "k_norm", hd, dev), eps, int(neox), n_rot,
-          _f32(freqs, "freqs", n_rot // 2, dev), None if rope_pos is None else rope_pos.data_ptr(), n_axes, axes, kvt,
-          k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
-          _int32(page_table, "page_table", (n_seq, page_table.shape[1]), dev), n_seq, page_table.shape[1],
-          None if seq is None else _int32(seq, "seq", (n,), dev), _int32(pos, "pos", (n,), dev), op, os_,
-          _status(status, dev))
+    st = L.load().sfk_qk_norm_rope_append(
+        io, qp, qs, kp, ks, vp, vs, n, heads, kvh, hd, None if q_norm is None else _f32(q_norm, "q_norm", hd, dev),
+        None if k_norm is None else _f32(k_norm, "k_norm", hd, dev), eps, neox, n_rot, fp, rp, n_axes, axes, kvt,
+        k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
+        _int32(page_table, "page_table", (n_seq, max_pages), dev), n_seq, max_pages,
+        None if seq is None else _int32(seq, "seq", (n,), dev), _int32(pos, "pos", (n,), dev), op, os_,
+        None if status is None else _status(status, dev), _stream_of(dev))
+    if st:
+        L.check(st)
     return out
 
 
@@ -308,15 +321,22 @@ def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     positions[t] (negative: padding, zeros) over the keys it sees: j <= p and,
     with window > 0, j > p - window or j < n_sink.  Returns [n_seq][Hq * hd]."""
     dev = _cuda_device(q, "q")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return attn_decode_window(q, k_pages, v_pages, page_table, positions, window=window, n_sink=n_sink,
+                                      scale=scale, out=out, status=status)
     kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
     heads, qp, qs, out, op = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
-    n = q.shape[0]
-    ws_bytes = _decode_workspace(dev, n, heads, kvh, hd, page_table.shape[1], window, n_sink)
+    n, max_pages = q.shape[0], page_table.shape[1]
+    ws_bytes = _decode_workspace(dev, n, heads, kvh, hd, max_pages, window, n_sink)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    _call(dev, L.load().sfk_attn_decode_window, _ROW_TYPES[q.dtype], qp, qs, kvt, k_pages.data_ptr(),
-          v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
-          page_table.shape[1], _int32(positions, "positions", (n,), dev), n, heads, kvh, hd, scale, window, n_sink,
-          op, None if ws is None else ws.data_ptr(), ws_bytes, _status(status, dev))
+    st = L.load().sfk_attn_decode_window(
+        _ROW_TYPES[q.dtype], qp, qs, kvt, k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
+        _int32(page_table, "page_table", (n, max_pages), dev), max_pages, _int32(positions, "positions", (n,), dev), n,
+        heads, kvh, hd, scale, window, n_sink, op, None if ws is None else ws.data_ptr(), ws_bytes,
+        None if status is None else _status(status, dev), _stream_of(dev))
+    if st:
+        L.check(st)
     return out
 
 
@@ -329,11 +349,18 @@ def attn_prefill_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     the cache; each attends over the keys it sees (attn_decode_window).
     Returns [tokens][Hq * hd]; rows of no sequence are not written."""
     dev = _cuda_device(q, "q")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return attn_prefill_window(q, k_pages, v_pages, page_table, q_start, kv_len, window=window, n_sink=n_sink,
+                                       scale=scale, out=out, status=status)
     kvt, kvh, hd = _pools(k_pages, v_pages, page_table, dev)
     heads, qp, qs, out, op = _attn_rows(q, k_pages, kvh, hd, window, n_sink, out, dev)
-    n = page_table.shape[0]
-    _call(dev, L.load().sfk_attn_prefill_window, _ROW_TYPES[q.dtype], qp, qs, q.shape[0], kvt, k_pages.data_ptr(),
-          v_pages.data_ptr(), k_pages.shape[0], _int32(page_table, "page_table", (n, page_table.shape[1]), dev),
-          page_table.shape[1], _int32(q_start, "q_start", (n + 1,), dev), _int32(kv_len, "kv_len", (n,), dev), n, heads,
-          kvh, hd, scale, window, n_sink, op, _status(status, dev))
+    n, max_pages = page_table.shape
+    st = L.load().sfk_attn_prefill_window(
+        _ROW_TYPES[q.dtype], qp, qs, q.shape[0], kvt, k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
+        _int32(page_table, "page_table", (n, max_pages), dev), max_pages, _int32(q_start, "q_start", (n + 1,), dev),
+        _int32(kv_len, "kv_len", (n,), dev), n, heads, kvh, hd, scale, window, n_sink, op,
+        None if status is None else _status(status, dev), _stream_of(dev))
+    if st:
+        L.check(st)
     return out
