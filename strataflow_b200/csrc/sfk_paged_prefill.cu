@@ -14,8 +14,8 @@ namespace sfk {
 namespace {
 
 // ---- CUDA cores: any cache type ------------------------------------------------------
-// For f32 caches, 32-bit rows over a bf16 cache and heads of 256; the other prompts
-// go to sfk_paged_prefill_tc.cu.  Bound by the multiply-adds and their shared loads
+// For f32 caches, and 32-bit rows over a bf16 cache or with heads of 256; the other
+// prompts go to sfk_paged_prefill_tc.cu.  Bound by the multiply-adds and their shared loads
 // (8 loads of 16 bytes to 64 multiply-adds): 2048 tokens, 32 heads of 128 over 8, f32:
 // 1.51 ms, 23 TFLOP/s.
 // 64 rows x 64 keys per step, 256 threads as 16 x 16: thread (ty, tx) owns rows

@@ -22,6 +22,10 @@
 // One thread issues in about 30 cycles a product and 100 a wait: Q K^T and P V
 // by one thread were what the kernel waited for.
 //
+// Heads of 256 take one row tile: its O is half of TMEM, and q and two stages of K and
+// V of 80 keys fill shared memory.  4096 tokens, 16 heads over 8 (137 GFLOP): 157 us,
+// 0.87 PFLOP/s, where the CUDA cores reach 13 TFLOP/s.
+//
 // Bound by the tensor core and the exponentials, which take about as long, under
 // the card's power limit: 2048 tokens at 30000 keys, 32 heads of 128 over 8, bf16
 // (974 GFLOP): 810 us in a burst (1.20 PFLOP/s), 920 back to back at 1.6 GHz and 1000 W
@@ -65,10 +69,11 @@ struct Cfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;  // head width in shared memory (the copy fills with zeros)
   static constexpr int HALVES = HDP / 64;        // 128-byte column blocks
   static constexpr int NS = SPLIT ? 2 : 1;       // terms of q and P
-  static constexpr int TILES = SPLIT ? 1 : 2;    // row tiles per CTA
+  static constexpr int TILES = SPLIT || HD > 128 ? 1 : 2;  // row tiles per CTA
+  static constexpr int OBUF = SPLIT ? 2 : TILES;           // O tiles
   static constexpr int ROWS = TILES * TM;
-  // Keys per tile: S (TK columns), P (TK / 2 a term) and O (HDP) of two row tiles, or of one with a second O, share
-  // the 512 columns of TMEM
+  // Keys per tile: S (TK columns), P (TK / 2 a term) and O (HDP) of two row tiles, or of one (with a second O; with an
+  // O of 256), share the 512 columns of TMEM
   static constexpr int TK = HDP == 64 || SPLIT ? 96 : 80;
   static constexpr int PPT = TK / PG;            // pages per key tile
   static constexpr int TILE = TK * HDP * 2;      // bytes of a K or V tile
@@ -85,7 +90,7 @@ struct Cfg {
   static constexpr int REG_SOFTMAX = 184, REG_OTHER = 136;
   static_assert(2 * 128 * REG_SOFTMAX + 128 * REG_OTHER <= TT * 168, "register split above the launch's");
   // TMEM columns
-  static constexpr int P0 = TILES * TK, PCOLS = TK / 2 * NS, O0 = 512 - 2 * HDP;
+  static constexpr int P0 = TILES * TK, PCOLS = TK / 2 * NS, O0 = 512 - OBUF * HDP;
   static_assert(P0 + TILES * PCOLS <= O0 && STAGES >= 2 && TK % PG == 0, "tile sizes");
 };
 
@@ -445,16 +450,20 @@ __global__ void __launch_bounds__(TT, 1)
             }
           }
         } else {
-          Raw8<KV> raw[LR];
+          constexpr int B = LR < 16 ? LR : 16;
+#pragma unroll 1
+          for (int i0 = 0; i0 < LR; i0 += B) {
+            Raw8<KV> raw[B];
 #pragma unroll
-          for (int i = 0; i < LR; ++i) {
-            const int64_t at = __shfl_sync(0xffffffffu, my_q, i * RI + lane / LR);
-            raw[i].w[0] = make_uint4(0, 0, 0, 0);
-            if (at >= 0) load8(raw[i], static_cast<const KV*>(p.q) + at + ch * 8, p.q_vec);
+            for (int i = 0; i < B; ++i) {
+              const int64_t at = __shfl_sync(0xffffffffu, my_q, (i0 + i) * RI + lane / LR);
+              raw[i].w[0] = make_uint4(0, 0, 0, 0);
+              if (at >= 0) load8(raw[i], static_cast<const KV*>(p.q) + at + ch * 8, p.q_vec);
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+              *reinterpret_cast<uint4*>(slot(wrow % TM + (i0 + i) * RI + lane / LR, ch)) = raw[i].w[0];
           }
-#pragma unroll
-          for (int i = 0; i < LR; ++i)
-            *reinterpret_cast<uint4*>(slot(wrow % TM + i * RI + lane / LR, ch)) = raw[i].w[0];
         }
         if constexpr (HDP > HD) {  // dims past the head
 #pragma unroll
@@ -936,6 +945,8 @@ template <class KV, bool SPLIT>
 cudaError_t launch_hd(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStream_t st) {
   if (hd == 32) return launch_t<KV, 32, SPLIT>(p, kv, sm_count, st);
   if (hd == 64) return launch_t<KV, 64, SPLIT>(p, kv, sm_count, st);
+  if constexpr (!SPLIT)
+    if (hd == 256) return launch_t<KV, 256, false>(p, kv, sm_count, st);
   return launch_t<KV, 128, SPLIT>(p, kv, sm_count, st);
 }
 
@@ -944,7 +955,7 @@ cudaError_t launch_hd(WindowAttnParams& p, int kv, int hd, int sm_count, cudaStr
 bool prefill_tc_takes(const WindowAttnParams& p, int kv, int hd) {
   const int64_t rows = (int64_t)p.n_pages * p.n_head_kv * PG;
   const int64_t tiles = (int64_t)p.n_tok * (p.n_head / p.n_head_kv) / TM + p.n_seq;
-  if (hd > 128 || rows >= 0x7fffffff || tiles * p.n_head_kv * 8 > 0x7fffffff) return false;
+  if ((hd > 128 && p.io == EL_F32) || rows >= 0x7fffffff || tiles * p.n_head_kv * 8 > 0x7fffffff) return false;
   return kv == EL_F16 || (kv == EL_BF16 && p.io == EL_BF16);
 }
 

@@ -406,6 +406,15 @@ def test_prefill_many_sequences(cuda, io, kv, hd):
     run_prefill(n_qs, [(i * 37) % 90 for i in range(300)], 4, 2, hd, io, kv, 20, 1)
 
 
+@pytest.mark.parametrize("io,kv", [(F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("n_qs,pasts,window,n_sink", [
+    ([1200], [0], 0, 0), ([700], [1500], 500, 200), ([5], [3000], 0, 0), ([33, 1, 0, 129], [1000, 4000, 3, 79], 900, 3)])
+def test_prefill_wide_heads(cuda, io, kv, n_qs, pasts, window, n_sink):
+    """Heads of 256 of 16-bit rows, one row tile to a CTA: several tiles, split keys, ragged ends."""
+    run_prefill(n_qs, pasts, 8, 2, 256, io, kv, window, n_sink, seed=len(n_qs) + window)
+    run_prefill(n_qs, pasts, 3, 3, 256, io, kv, window, n_sink, seed=7)
+
+
 def test_prefill_long_context_keeps_32_bits(cuda):
     """32-bit rows at 30000 keys: within the bound, and free of the drift that one accumulator over all keys shows."""
     from strataflow_b200 import ops
@@ -432,7 +441,7 @@ def test_prefill_large_scores(cuda):
 
 
 @pytest.mark.parametrize("n_q,past", [(200, 60), (130, 700)])
-@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 128)])
+@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 128), (F16, F16, 256)])
 def test_prefill_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd, n_q, past):
     """A key whose value is infinite or NaN touches the rows that see it and no other, in the same tile too."""
     from strataflow_b200 import ops
