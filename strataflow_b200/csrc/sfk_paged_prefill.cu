@@ -8,6 +8,8 @@
 // matrix: row r of a (sequence, kv head) is token r / G, head r % G.  A CTA
 // takes a tile of rows and walks the key tiles its rows see with a running
 // maximum, sum and output per row (f32).
+#include <type_traits>
+
 #include "sfk_paged.cuh"
 
 namespace sfk {
@@ -15,9 +17,10 @@ namespace {
 
 // ---- CUDA cores: any cache type ------------------------------------------------------
 // For f32 caches, and 32-bit rows over a bf16 cache or with heads of 256; the other
-// prompts go to sfk_paged_prefill_tc.cu.  Bound by the multiply-adds and their shared loads
-// (8 loads of 16 bytes to 64 multiply-adds): 2048 tokens, 32 heads of 128 over 8, f32:
-// 1.51 ms, 23 TFLOP/s.
+// prompts go to sfk_paged_prefill_tc.cu.  Bound by the multiply-adds, two to an
+// instruction, and the softmax between them: 2048 tokens, 32 heads of 128 over 8, f32:
+// 1.30 ms, 27 TFLOP/s; at 8048 keys 6.9 ms, 34 TFLOP/s.  (One multiply-add an instruction
+// and one CTA to an SM: 1.52 and 9.0 ms.)
 // 64 rows x 64 keys per step, 256 threads as 16 x 16: thread (ty, tx) owns rows
 // ty + 16 i, keys tx + 16 j of the scores and dims 4 tx .. 4 tx + 3 of each 64
 // of the output.  Everything is f32 in shared memory, rows padded by 16 bytes.
@@ -25,12 +28,16 @@ constexpr int FR = 64, FK = 64, FT = 256;
 
 template <int HD>
 struct FmaSmem {
-  float q[FR][HD + 4], k[FK][HD + 4], v[FK][HD + 4];
+  // Of wide heads K and V take turns in one place, so that two CTAs of 128 fit an SM and one loads while the other
+  // multiplies; of narrow ones they arrive together, in one round trip.
+  static constexpr bool TURNS = HD >= 128;
+  float q[FR][HD + 4], k[FK][HD + 4], v_own[TURNS ? 1 : FK][HD + 4];
   float p[FR][FK + 4];
+  __device__ float (*v())[HD + 4] { return TURNS ? k : v_own; }
 };
 
 template <class KV, int HD>
-__global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__ WindowAttnParams p) {
+__global__ void __launch_bounds__(FT, HD > 128 ? 1 : 2) prefill_fma_kernel(const __grid_constant__ WindowAttnParams p) {
   using Smem = FmaSmem<HD>;
   constexpr int NC = (HD + 63) / 64;  // chunks of 64 output dims
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -54,7 +61,8 @@ __global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__
   sp.n = 0;
   if (p_hi >= 0) sp = seen_pages(p_lo, p_hi, p.window, p.n_sink);
   int pos[4];
-  float m[4], l[4], o[4][NC][4];
+  float m[4], l[4];
+  uint64_t o[4][NC][2];  // two dims each
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty + 16 * i;
@@ -62,68 +70,82 @@ __global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
+    for (int c = 0; c < NC; ++c) o[i][c][0] = o[i][c][1] = both(0.f);
   }
-  for (int i0 = 0; i0 < sp.n; i0 += FK / PG) {
-    __syncthreads();
-    // four pages of keys and values; what no row sees is zero
+  // Four pages of one pool, or of both; what no row sees is zero.  Returns whether a number of this thread's last pool
+  // is infinite or NaN.
+  auto load = [&](int i0, const void* pages, float (*dst)[HD + 4], auto both_pools) {
+    constexpr int N = decltype(both_pools)::value ? 2 : 1;
+    bool odd = false;
+#pragma unroll 2
     for (int i = tid; i < FK * HD / 8; i += FT) {
       const int key = i / (HD / 8), d = i % (HD / 8) * 8;
-      float a[8] = {}, b[8] = {};
+      float a[N][8] = {};
       const int e = i0 + key / PG;
       if (e < sp.n && sp.page(e) * PG + key % PG <= p_hi) {
         const int id = p.page_table[(int64_t)t.seq * p.max_pages + sp.page(e)];
         if (id >= 0 && id < p.n_pages) {
           const int64_t off = (((int64_t)id * p.n_head_kv + hk) * PG + key % PG) * HD + d;
-          Raw8<KV> ra, rb;
-          load8(ra, static_cast<const KV*>(p.k_pages) + off, true);
-          load8(rb, static_cast<const KV*>(p.v_pages) + off, true);
-          unpack8(ra, a);
-          unpack8(rb, b);
+          Raw8<KV> raw[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) load8(raw[k], static_cast<const KV*>(k ? p.v_pages : pages) + off, true);
+#pragma unroll
+          for (int k = 0; k < N; ++k) unpack8(raw[k], a[k]);
         } else {
           report(p.status, ERR_BAD_PAGE);
         }
       }
 #pragma unroll
-      for (int x = 0; x < 8; x += 4) {
-        *reinterpret_cast<float4*>(&sm.k[key][d + x]) = make_float4(a[x], a[x + 1], a[x + 2], a[x + 3]);
-        *reinterpret_cast<float4*>(&sm.v[key][d + x]) = make_float4(b[x], b[x + 1], b[x + 2], b[x + 3]);
+      for (int k = 0; k < N; ++k) {
+        float* to = k ? &sm.v()[key][d] : &dst[key][d];
+        *reinterpret_cast<float4*>(to) = make_float4(a[k][0], a[k][1], a[k][2], a[k][3]);
+        *reinterpret_cast<float4*>(to + 4) = make_float4(a[k][4], a[k][5], a[k][6], a[k][7]);
       }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) odd = odd || !(fabsf(a[N - 1][x]) < INFINITY);
     }
+    return odd;
+  };
+  const int row_lo = n_rows < FR ? -1 : t.past + t.row0 / G;  // a row of the tile that is none sees nothing
+  for (int i0 = 0; i0 < sp.n; i0 += FK / PG) {
     __syncthreads();
-    float s[4][4];
+    bool odd = load(i0, p.k_pages, sm.k, std::bool_constant<!Smem::TURNS>());
+    odd = __syncthreads_or(odd);
+    uint64_t s2[4][4];  // the sums of even and of odd dims
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+      for (int j = 0; j < 4; ++j) s2[i][j] = both(0.f);
 #pragma unroll 4
     for (int d = 0; d < HD; d += 4) {
-      float4 q[4], k[4];
+      ulonglong2 q[4], k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(&sm.q[ty + 16 * i][d]);
+      for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const ulonglong2*>(&sm.q[ty + 16 * i][d]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(&sm.k[tx + 16 * j][d]);
+      for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const ulonglong2*>(&sm.k[tx + 16 * j][d]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(q[i].x, k[j].x, s[i][j]);
-          s[i][j] = fmaf(q[i].y, k[j].y, s[i][j]);
-          s[i][j] = fmaf(q[i].z, k[j].z, s[i][j]);
-          s[i][j] = fmaf(q[i].w, k[j].w, s[i][j]);
-        }
+        for (int j = 0; j < 4; ++j) s2[i][j] = fma2(q[i].y, k[j].y, fma2(q[i].x, k[j].x, s2[i][j]));
     }
+    if (Smem::TURNS) {
+      __syncthreads();
+      odd = load(i0, p.v_pages, sm.v(), std::false_type());
+    }
+    // all keys seen by all rows (7.2 ms for the 8048 keys below where each key asks)
+    const bool inner = i0 >= sp.sink && i0 + FK / PG <= sp.n && sp.page(i0 + FK / PG - 1) * PG + PG - 1 <= row_lo &&
+                       (p.window == 0 || sp.page(i0) * PG > p_hi - p.window);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float mx = m[i];
+      float mx = m[i], s[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int e = i0 + j;  // key tx of page entry i0 + j
-        const bool see = e < sp.n && key_seen(sp.page(e) * PG + tx, pos[i], p.window, p.n_sink);
-        s[i][j] = see ? s[i][j] * p.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, s[i][j]);
+        const bool see = inner || (e < sp.n && key_seen(sp.page(e) * PG + tx, pos[i], p.window, p.n_sink));
+        float even, odd;
+        unpair(s2[i][j], even, odd);
+        s[j] = see ? (even + odd) * p.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[j]);
       }
 #pragma unroll
       for (int d = 1; d < 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
@@ -132,39 +154,45 @@ __global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__
       m[i] = mx;
       l[i] *= f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][c][e] *= f;
+      for (int c = 0; c < NC; ++c) {
+        o[i][c][0] = mul2(o[i][c][0], both(f));
+        o[i][c][1] = mul2(o[i][c][1], both(f));
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float pr = exp2_approx(s[i][j] - ms);
+        const float pr = exp2_approx(s[j] - ms);
         l[i] += pr;
         sm.p[ty + 16 * i][tx + 16 * j] = pr;
       }
     }
-    __syncwarp();  // rows ty + 16 i belong to one half of a warp
-    for (int k0 = 0; k0 < FK; k0 += 4) {
-      float pr[4][4];
+    if (Smem::TURNS) odd = __syncthreads_or(odd);  // V has arrived
+    else __syncwarp();                             // rows ty + 16 i belong to one half of a warp
+    // A masked key's weight is 0, which takes its value out unless that is infinite or NaN: only then each product
+    // asks (2048 tokens at 8048 keys, 32 heads of 128, f32: 6.8 ms, 8.7 ms where all ask).
+    auto add = [&](auto ask) {
+#pragma unroll 1
+      for (int k0 = 0; k0 < FK; k0 += 4) {
+        float pr[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(pr[i]) = *reinterpret_cast<const float4*>(&sm.p[ty + 16 * i][k0]);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (HD < 64 && tx >= HD / 4) continue;
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(pr[i]) = *reinterpret_cast<const float4*>(&sm.p[ty + 16 * i][k0]);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-          const float4 v = *reinterpret_cast<const float4*>(&sm.v[k0 + kk][c * 64 + tx * 4]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (pr[i][kk] != 0.f) {  // a masked key's value, whatever it holds, is not used
-              o[i][c][0] = fmaf(pr[i][kk], v.x, o[i][c][0]);
-              o[i][c][1] = fmaf(pr[i][kk], v.y, o[i][c][1]);
-              o[i][c][2] = fmaf(pr[i][kk], v.z, o[i][c][2]);
-              o[i][c][3] = fmaf(pr[i][kk], v.w, o[i][c][3]);
-            }
+          for (int c = 0; c < NC; ++c) {
+            if (HD < 64 && tx >= HD / 4) continue;
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.v()[k0 + kk][c * 64 + tx * 4]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!decltype(ask)::value || pr[i][kk] != 0.f) {
+                o[i][c][0] = fma2(both(pr[i][kk]), v.x, o[i][c][0]);
+                o[i][c][1] = fma2(both(pr[i][kk]), v.y, o[i][c][1]);
+              }
           }
         }
       }
-    }
+    };
+    if (odd) add(std::true_type());
+    else add(std::false_type());
     __syncwarp();
   }
 #pragma unroll
@@ -177,10 +205,13 @@ __global__ void __launch_bounds__(FT) prefill_fma_kernel(const __grid_constant__
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (HD < 64 && tx >= HD / 4) continue;
+      float x[4];
+      unpair(o[i][c][0], x[0], x[1]);
+      unpair(o[i][c][1], x[2], x[3]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         store_elem(p.out, ((int64_t)(t.q0 + tok) * p.n_head + h) * HD + c * 64 + tx * 4 + e,
-                   pos[i] >= 0 ? o[i][c][e] / l[i] : 0.f, p.io);
+                   pos[i] >= 0 ? x[e] / l[i] : 0.f, p.io);
     }
   }
 }

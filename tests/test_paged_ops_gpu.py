@@ -323,7 +323,8 @@ def test_decode_strided_queries_streams_and_repeats(cuda):
     assert torch.equal(other.view_as(got), got)
 
 
-@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (BF16, BF16, 128), (F16, F16, 256)])
+@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (BF16, BF16, 128), (F16, F16, 256),
+                                      (F32, F32, 128), (F32, BF16, 256)])
 def test_decode_bad_pages_and_positions(cuda, io, kv, hd):
     from strataflow_b200 import lib as L
     from strataflow_b200 import ops
@@ -441,7 +442,8 @@ def test_prefill_large_scores(cuda):
 
 
 @pytest.mark.parametrize("n_q,past", [(200, 60), (130, 700)])
-@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 128), (F16, F16, 256)])
+@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 128), (F16, F16, 256),
+                                      (F32, F32, 128), (F32, BF16, 256)])
 def test_prefill_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd, n_q, past):
     """A key whose value is infinite or NaN touches the rows that see it and no other, in the same tile too."""
     from strataflow_b200 import ops
