@@ -245,15 +245,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // bits of x + 1.5 2^23), 2^f on [-1/2, 1/2] by a polynomial of least relative
 // error (Lawson's iteration), n added to the exponent.  Relative error 7.5e-5 at
 // degree 3, 2.7e-6 at degree 4: well below the rounding of P to bf16 (2^-8) and
-// f16 (2^-11).  x below -126 gives 2^-126.
-template <int DEG>
+// f16 (2^-11).  x below -126 gives 2^-126, which is 0 in f16.  bf16 holds it, and a masked key's value may be
+// 3e38: there x2 comes 24 larger, and the factor 2^-24 at the end flushes all below 2^-126 to 0.
+constexpr float POLY_UP = 24.f;
+template <bool BF16>
 __device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
   unpair(x2, x, y);
   x2 = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
   const uint64_t t = add2(x2, both(12582912.f));
   const uint64_t f = fma2(add2(t, both(-12582912.f)), both(-1.f), x2);
   uint64_t r;
-  if constexpr (DEG == 3) {
+  if constexpr (BF16) {
     r = fma2(both(0.0551716685295105f), f, both(0.2426111251115799f));
     r = fma2(r, f, both(0.6932609677314758f));
     r = fma2(r, f, both(0.9999280571937561f));
@@ -268,6 +270,7 @@ __device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
   unpair(t, u, v);
   x = __int_as_float(__float_as_int(a) + (__float_as_int(u) << 23));
   y = __int_as_float(__float_as_int(b) + (__float_as_int(v) << 23));
+  if constexpr (BF16) unpair(mul2_ftz(pair(x, y), both(1.f / (1 << (int)POLY_UP))), x, y);
 }
 
 // ---- rows with a non-finite output ------------------------------------------------------
@@ -624,17 +627,18 @@ __global__ void __launch_bounds__(TT, 1)
             if (lane == 0) mbar_arrive(&c->f_full[n % 4]);
           }
           const float neg = BIAS - (m == -INFINITY ? 0.f : m);
-          const uint64_t scale2 = both(scale), neg2 = both(neg);
+          const uint64_t scale2 = both(scale), neg2 = both(neg), up2 = both(neg + POLY_UP);
           uint64_t sum2 = 0;
 #pragma unroll
           for (int b = 0; b < PPT; ++b) {  // 16 keys: 8 columns of P
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, neg2);
+              const bool poly = (k * 3) % 8 < C::POLY_OF_8;
+              const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, BF16 && poly ? up2 : neg2);
               float x, y;
-              if ((k * 3) % 8 < C::POLY_OF_8) {
-                exp2_poly<BF16 ? 3 : 4>(x2, x, y);
+              if (poly) {
+                exp2_poly<BF16>(x2, x, y);
               } else {
                 unpair(x2, x, y);
                 x = exp2_approx(x);

@@ -464,6 +464,29 @@ def test_prefill_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd, n_q, past):
     check(got.view_as(want)[~touched], want[~touched], tol[~touched])
 
 
+@pytest.mark.parametrize("n_q,past", [(200, 60), (130, 700)])
+@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, BF16, 128), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 32),
+                                      (BF16, BF16, 64), (BF16, BF16, 128), (BF16, BF16, 256)])
+def test_prefill_largest_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd, n_q, past):
+    """The largest finite values of the cache's type at keys that some rows of a tile see and others do not: a weight
+    of 2^-126 instead of 0 would already add 4."""
+    from strataflow_b200 import ops
+    window, n_sink = n_q * 9 // 20, 2
+    q, c, start, kv_len, _ = run_prefill([n_q], [past], 8, 2, hd, io, kv, window, n_sink, gap=0)
+    first = past + n_q * 9 // 20
+    bad = range(first, first + 12)
+    for j in bad:
+        c.v[c.table[0, j // PG], :, j % PG] = torch.finfo(kv).max
+    got = ops.attn_prefill_window(q, c.k, c.v, c.table, start, kv_len, window=window, n_sink=n_sink)
+    p = past + torch.arange(n_q, device="cuda")
+    touched = (p >= bad[0]) & (p < bad[-1] + window)
+    assert touched.any() and not touched.all()
+    want, tol, absv = reference(q, c.keys[0], c.values[0], range(past, past + n_q), window, n_sink)
+    if io != F32:
+        tol = tol + half_step(io) * want.abs() + weight_tol(kv, absv)
+    check(got.view_as(want)[~touched], want[~touched], tol[~touched])
+
+
 def test_prefill_tokens_before_the_first_position(cuda):
     """kv_len below the tokens: the first ones have negative positions and give zeros."""
     from strataflow_b200 import ops
