@@ -474,6 +474,12 @@ __device__ __forceinline__ void two_terms(float x, float y, uint32_t& hi, uint32
   }
 }
 
+// The sum of the two terms' products.  An infinite key or value times the second term is infinite of either sign, or
+// NaN: the first term's product alone is what the formula gives.
+__device__ __forceinline__ float add_terms(float first, float second) {
+  return fabsf(first) < INFINITY ? first + second : first;
+}
+
 template <int HD, int DW>
 struct MmaCfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;    // head width in a slot (the copy fills with zeros)
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
         mma16816<BF16>(s1, a1, k1.z, k1.w);
       }
     // keys 2t, 2t+1, 2t+8, 2t+9 of head g
-    float x[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+    float x[4] = {add_terms(s0[0], s0[2]), add_terms(s0[1], s0[3]), add_terms(s1[0], s1[2]), add_terms(s1[1], s1[3])};
     const bool gone = bad >> (k % S) & 1;
     const bool edge = gone || j0 + PG - 1 > w.pos || (p.window > 0 && j0 <= w.pos - p.window);
     bool see[4];
@@ -695,8 +701,8 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = b * 64 + 16 * t + e;  // and d + 8
-      if (d < HD) sm.join.o[warp][g][d] = o[b * 8 + e][0] + o[b * 8 + e][2];
-      if (d + 8 < HD) sm.join.o[warp][g][d + 8] = o[b * 8 + e][1] + o[b * 8 + e][3];
+      if (d < HD) sm.join.o[warp][g][d] = add_terms(o[b * 8 + e][0], o[b * 8 + e][2]);
+      if (d + 8 < HD) sm.join.o[warp][g][d + 8] = add_terms(o[b * 8 + e][1], o[b * 8 + e][3]);
     }
   join_and_store(sm.join, p, w.seq, w.head0, w.n_rows, w.pos >= 0);
 }

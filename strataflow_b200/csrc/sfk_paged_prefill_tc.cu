@@ -158,17 +158,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
       R16("f", v, 0)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[64]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : R32("=f", v, 0), R32("=f", v, 32)
-      : "r"(addr), "r"(addr + 32)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[80]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -194,6 +183,11 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[96]) {
       : R32("=f", v, 0), R32("=f", v, 32), R32("=f", v, 64)
       : "r"(addr), "r"(addr + 32), "r"(addr + 64)
       : "memory");
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), R8("r", v, 0)
@@ -557,8 +551,9 @@ __global__ void __launch_bounds__(TT, 1)
           }
         }
         __syncwarp();
-        // an infinite or NaN value that this row may not see; a sum that is not finite is the row's own
-        unsigned again = __ballot_sync(0xffffffffu, live && pos >= 0 && !finite && l < INFINITY);
+        // an infinite or NaN value that this row may not see; a sum that is not finite is the row's own, unless the two
+        // terms of q met an infinite key with two signs
+        unsigned again = __ballot_sync(0xffffffffu, live && pos >= 0 && !finite && (SPLIT || l < INFINITY));
         while (again) {
           const int src = __ffs(again) - 1;
           again &= again - 1;
@@ -596,8 +591,8 @@ __global__ void __launch_bounds__(TT, 1)
 #pragma unroll
           for (int k = 4; k < TK; k += 4)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], s[k + i]);
-          float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            for (int i = 0; i < 4; ++i) m4[i] = max_nan(m4[i], s[k + i]);
+          float mx = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
           // O is complete and P may be written again (mostly long since)
           if (n > 0) {
             if (!(ok = wait_warp(&c->pv_done[w], (n - 1) & 1, c))) break;
@@ -605,8 +600,9 @@ __global__ void __launch_bounds__(TT, 1)
           }
           mx *= scale;
           float f = 1.f;
-          if (__any_sync(0xffffffffu, mx > m + RAISE || m == -INFINITY)) {
-            const float mn = fmaxf(mx, m);
+          if (__any_sync(0xffffffffu, !(mx <= m + RAISE))) {
+            // a row that saw a score of NaN or +inf is NaN, by its m: the polynomial below does not carry these on
+            const float mn = max_nan(mx, m) < INFINITY ? fmaxf(mx, m) : NAN;
             f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
             m = mn;
             l *= f;
@@ -891,7 +887,7 @@ __global__ void __launch_bounds__(TT, 1)
             finite = finite && fabsf(o[j][e]) < INFINITY;
             store_elem(p.out, ((int64_t)(t.q0 + tok) * p.n_head + h) * HD + lane * E + e, sees ? o[j][e] / lr : 0.f, p.io);
           }
-          if (__any_sync(0xffffffffu, !finite) && sees && lr < INFINITY) recompute_row<KV, HD>(p, t, hk, r);
+          if (__any_sync(0xffffffffu, !finite) && sees && (SPLIT || lr < INFINITY)) recompute_row<KV, HD>(p, t, hk, r);
         }
       }
     }

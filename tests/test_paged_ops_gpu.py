@@ -348,6 +348,38 @@ def test_decode_bad_pages_and_positions(cuda, io, kv, hd):
         assert torch.equal(got[1], good[1])
 
 
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [32, 128, 256])
+@pytest.mark.parametrize("n", [40, 700, 20000])
+def test_decode_infinite_and_nan_keys_and_values(cuda, io, kv, hd, n):
+    """Of keys that are seen: what the formula gives, in the heads of the key's kv head alone."""
+    from strataflow_b200 import ops
+    q, c, pos, _ = run_decode([n], 8, 2, hd, io, kv, 0, 0)
+    j, x0 = n - 7, q[0, :4, 0].float()
+    at = (c.table[0, j // PG], 0, j % PG)
+    k, v = c.k[at].clone(), c.v[at].clone()
+
+    def run():
+        return ops.attn_decode_window(q, c.k, c.v, c.table, pos).view(8, hd).float()
+
+    good = run()
+    c.v[at][3] = math.inf
+    got = run()
+    assert (got[:4, 3] == math.inf).all() and torch.equal(got[4:], good[4:])
+    others = [d for d in range(hd) if d != 3]
+    assert torch.equal(got[:, others], good[:, others])
+    c.v[at] = v
+    c.k[at] = 0
+    for x in (math.inf, -math.inf, math.nan):
+        c.k[at][0] = x
+        got = run()
+        s = x * x0
+        assert got[:4][s != -math.inf].isnan().all() and torch.equal(got[4:], good[4:])
+        low = s == -math.inf  # the key's weight is 0: as if it were not there
+        assert got[:4][low].isfinite().all()
+    c.k[at] = k
+
+
 # ---- prefill -------------------------------------------------------------------------------------------
 def run_prefill(n_qs, pasts, hq, hkv, hd, io, kv, window, n_sink, seed=0, scale=0.0, qscale=1.0, gap=3):
     """Ragged prompts with `gap` rows of no sequence before the first and behind the last."""
@@ -485,6 +517,31 @@ def test_prefill_largest_values_of_unseen_keys_do_not_leak(cuda, io, kv, hd, n_q
     if io != F32:
         tol = tol + half_step(io) * want.abs() + weight_tol(kv, absv)
     check(got.view_as(want)[~touched], want[~touched], tol[~touched])
+
+
+@pytest.mark.parametrize("n_q,past", [(200, 60), (130, 700)])
+@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, BF16, 128), (F32, F16, 128), (F16, F16, 64), (BF16, BF16, 64),
+                                      (BF16, BF16, 128), (BF16, BF16, 256)])
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 5, 7, 8, 14])
+def test_prefill_a_bad_key_shows_in_the_rows_that_see_it(cuda, io, kv, hd, n_q, past, at):
+    """A NaN in a key makes every row NaN that sees it, at any place of a tile, and no other row."""
+    from strataflow_b200 import ops
+    window = n_q * 9 // 20
+    q, c, start, kv_len, _ = run_prefill([n_q], [past], 8, 2, hd, io, kv, window, 0, gap=0)
+    j = (past + n_q * 9 // 20) // PG * PG + at
+    want, tol, absv = reference(q, c.keys[0], c.values[0], range(past, past + n_q), window, 0)
+    if io != F32:
+        tol = tol + half_step(io) * want.abs() + weight_tol(kv, absv)
+    p = past + torch.arange(n_q, device="cuda")
+    sees = (p >= j) & (p < j + window)
+    for x in (math.nan, math.inf):
+        c.k[c.table[0, j // PG], :, j % PG] = 0
+        c.k[c.table[0, j // PG], :, j % PG, 0] = x
+        got = ops.attn_prefill_window(q, c.k, c.v, c.table, start, kv_len, window=window).view_as(want)
+        # inf times q's first number: +inf (a NaN row), -inf (the key has weight 0) or, for a zero, NaN
+        nan = sees[:, None] & (torch.full_like(q[:, :, 0], x) * q[:, :, 0] != -math.inf)
+        assert got[nan].isnan().all() and not got[~nan].isnan().any()
+        check(got[~sees], want[~sees], tol[~sees])
 
 
 def test_prefill_tokens_before_the_first_position(cuda):
