@@ -575,7 +575,7 @@ SFK_API size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, i
  * (kv_len device), and token i of them sits at position kv_len[s] - n_q + i.
  * A token whose position is negative sees nothing and gives zeros; rows of q
  * outside every sequence are neither read nor written.
- * out: [n_tok][n_head * head_dim]. */
+ * out: [n_tok][n_head * head_dim], apart from q. */
 SFK_API sfk_status sfk_attn_prefill_window(int32_t io_type, const void *dev_q, int64_t q_stride, int32_t n_tok,
                                            int32_t kv_type, const void *dev_k_pages, const void *dev_v_pages,
                                            int32_t n_pages, const int32_t *dev_page_table, int32_t max_pages,

@@ -51,6 +51,8 @@ int current_sms() {
 
 constexpr int MAX_PAGES = 1 << 27;  // positions stay below 2^31
 
+constexpr float LOG2_E = 1.44269504088896340736f;
+
 // What the two attention entries share.
 sfk_status attn_args(const char* who, WindowAttnParams& a, int* kv, int32_t io_type, const void* q, int64_t q_stride,
                      int32_t kv_type, const void* kp, const void* vp, int32_t n_pages, const int32_t* table,
@@ -65,7 +67,7 @@ sfk_status attn_args(const char* who, WindowAttnParams& a, int* kv, int32_t io_t
     BAD("%s: %d heads over %d kv heads", who, n_head, n_head_kv);
   if (n_pages < 1 || max_pages < 1 || max_pages > MAX_PAGES) BAD("%s: pages (pool %d, table %d)", who, n_pages, max_pages);
   if (window < 0 || n_sink < 0) BAD("%s: window %d, sinks %d", who, window, n_sink);
-  if (!std::isfinite(scale) || scale < 0.f) BAD("%s: scale %g", who, (double)scale);
+  if (!std::isfinite(scale * LOG2_E) || scale < 0.f) BAD("%s: scale %g", who, (double)scale);
   if (!q || !kp || !vp || !table || !out) BAD("%s: null pointer", who);
   if (!aligned16(kp) || !aligned16(vp)) BAD("%s: page pools start on 16-byte boundaries", who);
   if (q_stride < (int64_t)n_head * hd) BAD("%s: q_stride %lld", who, (long long)q_stride);
@@ -81,7 +83,7 @@ sfk_status attn_args(const char* who, WindowAttnParams& a, int* kv, int32_t io_t
   a.n_head = n_head;
   a.n_head_kv = n_head_kv;
   a.page_table = table;
-  a.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)hd) : scale) * 1.44269504088896340736f;
+  a.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)hd) : scale) * LOG2_E;
   a.window = window;
   a.n_sink = n_sink;
   a.out = out;
@@ -209,6 +211,7 @@ sfk_status sfk_attn_prefill_window(int32_t io_type, const void* q, int64_t q_str
   if (!q_start || !kv_len) BAD("%s: null pointer", who);
   if (n_head_kv > 65535 || (int64_t)n_tok * (n_head / n_head_kv) > (1ll << 30))
     BAD("%s: %d tokens of %d heads in one call", who, n_tok, n_head);
+  if (out == q) BAD("%s: out is q", who);  // a row may be read again after others of its tile are written
   a.q_start = q_start;
   a.kv_len = kv_len;
   a.n_seq = n_seq;

@@ -806,7 +806,9 @@ cudaError_t launch_mma(WindowAttnParams& p, int kv, int sm_count, cudaStream_t s
 template <class KV, int HD>
 cudaError_t launch_16(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {
   if ((int64_t)p.n_pages * p.n_head_kv * PG >= 0x7fffffff) return launch_cc<KV, HD>(p, sm_count, st);  // beyond a map's rows
-  return p.io == EL_F32 ? launch_mma<KV, HD, true>(p, kv, sm_count, st) : launch_mma<KV, HD, false>(p, kv, sm_count, st);
+  if constexpr (std::is_same<KV, __half>::value)
+    if (p.io == EL_F32) return launch_mma<KV, HD, true>(p, kv, sm_count, st);
+  return launch_mma<KV, HD, false>(p, kv, sm_count, st);
 }
 
 template <int HD>

@@ -76,6 +76,14 @@ def test_prefill_refusals(sfk, kw, why):
     assert why in sfk.sfk_last_error()
 
 
+def test_scale_that_overflows_and_out_over_q(sfk):
+    for fn, base in (("sfk_attn_decode_window", DECODE), ("sfk_attn_prefill_window", PREFILL)):
+        assert call(sfk, fn, base, scale=3e38) == L.SFK_ERR_INVALID_ARGUMENT
+        assert b"scale" in sfk.sfk_last_error()
+    assert call(sfk, "sfk_attn_prefill_window", PREFILL, out=PREFILL["q"]) == L.SFK_ERR_INVALID_ARGUMENT
+    assert b"out is q" in sfk.sfk_last_error()
+
+
 def test_empty_calls_do_nothing(sfk):
     """No token, no sequence: fine without any pointer, and no launch."""
     assert call(sfk, "sfk_qk_norm_rope_append", APPEND, n=0, q=None, k=None, v=None, pos=None, out=None) == L.SFK_OK
