@@ -750,3 +750,67 @@ def test_wrapper_refusals(cuda):
             fn()
         assert e.value.status == L.SFK_ERR_INVALID_ARGUMENT, i
     torch.cuda.synchronize()
+
+
+def test_calls_right_behind_what_they_read_and_before_what_they_wrote(cuda):
+    """Each operator directly behind copies, fills, kernels and another stream's work that make its inputs, and in front
+    of kernels that change them: eager and captured, many steps without a host wait."""
+    from strataflow_b200 import ops
+    n, steps, hd = 3, 40, 64
+    g = gen(11)
+    rows = torch.randn((steps, n, 8 + 2 + 2, hd), generator=g, device="cuda")
+    freqs = ops.rope_freqs(hd)
+    table = torch.arange(1, 1 + n * 4, dtype=torch.int32, device="cuda").view(n, 4)
+    wide = torch.randn((1 << 23,), generator=g, device="cuda")
+
+    def fresh():
+        return dict(k=torch.zeros(1 + n * 4, 2, PG, hd, device="cuda", dtype=torch.float16),
+                    v=torch.zeros(1 + n * 4, 2, PG, hd, device="cuda", dtype=torch.float16),
+                    pos=torch.full((n,), -1, dtype=torch.int32, device="cuda"), x=torch.empty_like(rows[0]),
+                    q=torch.empty((n, 8, hd), device="cuda"), o=torch.empty((n, 8 * hd), device="cuda"),
+                    p=torch.empty((n, 8 * hd), device="cuda"), start=torch.arange(n + 1, dtype=torch.int32, device="cuda"),
+                    len=torch.zeros(n, dtype=torch.int32, device="cuda"), at=torch.zeros(1, dtype=torch.long, device="cuda"),
+                    sums=torch.zeros(n, 8 * hd, device="cuda"), side=torch.cuda.Stream())
+
+    def step(s, wait):
+        s["q"].zero_()
+        wide.mul_(1.0)  # a kernel that is still busy when the next launches arrive
+        s["x"].copy_(rows[s["at"]][0])
+        s["pos"].add_(1)
+        if wait:
+            torch.cuda.synchronize()
+        x = s["x"]
+        ops.qk_norm_rope_append(x[:, :8], x[:, 8:10], x[:, 10:], s["k"], s["v"], table, s["pos"], freqs=freqs, out=s["q"])
+        if wait:
+            torch.cuda.synchronize()
+        ops.attn_decode_window(s["q"], s["k"], s["v"], table, s["pos"], out=s["o"])
+        s["side"].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s["side"]):
+            torch.add(s["pos"], 1, out=s["len"])
+        torch.cuda.current_stream().wait_stream(s["side"])
+        if wait:
+            torch.cuda.synchronize()
+        ops.attn_prefill_window(s["q"], s["k"], s["v"], table, s["start"], s["len"], out=s["p"])
+        s["sums"].add_(s["o"]).add_(s["p"])
+        s["at"].add_(1)
+        s["x"].fill_(math.nan)
+        s["o"].fill_(math.nan)
+
+    want = fresh()
+    for _ in range(steps):
+        step(want, True)
+    eager = fresh()
+    for _ in range(steps):
+        step(eager, False)
+    torch.cuda.synchronize()
+    captured = fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(captured, False)
+    for _ in range(steps):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert want["sums"].isfinite().all() and int(want["at"]) == steps
+    for got in (eager, captured):
+        for name in ("sums", "k", "v", "pos", "q", "p"):
+            assert torch.equal(got[name], want[name]), name
