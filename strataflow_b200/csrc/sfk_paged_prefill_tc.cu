@@ -33,13 +33,17 @@
 // a window of 2048 (241 GFLOP): 262 us; a CTA walks 27 key tiles there and spends
 // a sixth of its time before the first and after the last.
 //
-// The running maximum m is only raised when a row outgrows it by 2^8: O is
-// rescaled then, by the row's own thread.  P then reaches 2^8, far inside both
-// 16-bit types, and the sum stays in 32 bits.
+// The running maximum m is only raised when a row outgrows it, in bf16 by 2^8: O
+// is rescaled then, by the row's own thread.  P is rounded once to the cache's
+// type, and the sum stays in 32 bits.  bf16 has the range of f32: P is 1 at m and
+// 2^8 at most.  f16's smallest step is 2^-24, and a long tail of weights far below
+// the row's largest would fall under it while the sum keeps them (one key 18 nats
+// above 30000 others: 0.95 of the tail lost): P is 2^11 at m, 2^15 at most, and a
+// weight is held to half a step of f16 or 2^-36 of the largest.
 //
 // 32-bit rows over an f16 cache (SPLIT): q, scaled by a power of two per row,
 // is the sum of two f16 numbers and so is each P (22 bits), and each product
-// is two.  P is 2^11 at m and 2^15 at most, so that its second part stays above
+// is two.  P's range is that of f16 rows, so that its second part too stays above
 // f16's smallest step.  A bf16 pair holds 16 bits only: that cache takes the
 // CUDA-core kernel.  One row tile per CTA then, and the second warpgroup keeps the
 // sum of the key tiles' O (below, at the sum).  512 tokens at 1012 keys, 32 heads of
@@ -476,8 +480,8 @@ __global__ void __launch_bounds__(TT, 1)
       }
       const uint32_t lanes = (uint32_t)(warp % 4) * 32 << 16;
       const uint32_t ts = tmem + lanes + w * TK, tp = tmem + lanes + C::P0 + w * C::PCOLS, to = tmem + lanes + C::O0 + w * HDP;
-      constexpr float RAISE = SPLIT ? 4.f : 8.f;   // log2 by which a row may outgrow m
-      constexpr float BIAS = SPLIT ? 11.f : 0.f;   // P = 2^BIAS at m
+      constexpr float RAISE = BF16 ? 8.f : 4.f;  // log2 by which a row may outgrow m
+      constexpr float BIAS = BF16 ? 0.f : 11.f;  // P = 2^BIAS at m
       bool ok = true;
       auto done = [&](uint64_t* bar) {  // what this warp's lanes did in TMEM so far
         fence_before();

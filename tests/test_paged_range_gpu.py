@@ -1,0 +1,79 @@
+"""GPU tests of the paged-cache attention at the ends of its range, against the formulas in 64 bits: weights far below
+the row's largest, the largest finite values at keys that are seen, infinite keys and values of tiny weight, contexts
+long enough that a lost page hides below an elementwise bound, tails of one accumulator.  Inputs, the 64-bit form and the
+elementwise bounds are those of test_paged_ops_gpu.py."""
+import math
+
+import pytest
+import torch
+
+from test_paged_ops_gpu import BF16, F16, F32, PG, TYPES, Cache, check, gen, half_step, reference, run_decode
+
+pytestmark = pytest.mark.gpu
+
+
+def one_number(n, hq, hkv, hd, io, kv, scores, seed, scale=0.125):
+    """(q, cache of one sequence) with score_j = scores[j] at every query: q is 1 in dim 0, keys hold nothing else."""
+    c = Cache([n], hkv, hd, kv, seed)
+    q = torch.randn((1, hq, hd), generator=gen(seed + 1), device="cuda").to(io)
+    q[..., 0] = 1
+    c.keys[0].zero_()
+    c.keys[0][..., 0] = (scores / scale).to(kv)[:, None]
+    store(c)
+    return q, c
+
+
+def store(c):
+    """The cache's pages from c.keys and c.values."""
+    for s, n in enumerate(c.lens):
+        j = torch.arange(n, device="cuda")
+        c.k[c.table[s, j // PG].long(), :, j % PG] = c.keys[s]
+        c.v[c.table[s, j // PG].long(), :, j % PG] = c.values[s]
+
+
+def prefill(q, c, past, **kw):
+    from strataflow_b200 import ops
+    n = q.shape[0]
+    start = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    return ops.attn_prefill_window(q, c.k, c.v, c.table, start, start[1:] + past, **kw).view_as(q)
+
+
+def decode(q, c, **kw):
+    from strataflow_b200 import ops
+    pos = torch.tensor(c.lens, dtype=torch.int32, device="cuda") - 1
+    return ops.attn_decode_window(q, c.k, c.v, c.table, pos, **kw).view_as(q)
+
+
+# ---- a dominant key over a long tail ---------------------------------------------------------------------
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n_q,hq", [(3, 4), (2400, 8)])
+def test_prefill_dominant_key_of_zero_value(cuda, io, kv, hd, n_q, hq):
+    """One key 18 nats above 30000 others, its value 0, the others' of one sign: the output is the tail alone, of which
+    each weight is 2^-26 of the largest.  With few tokens the keys are split, with 2400 they are not.
+
+    A weight w (1 at the largest) is rounded once: 16-bit rows to half a step of their type, or, in f16, to half of its
+    smallest step, where the largest weight stands for 2^11: 2^-36.  The rest is 32-bit arithmetic: the exponential and
+    the scores, below 18 here, to 2^-20 of a weight, and sums over n keys."""
+    n = 30000 + n_q
+    g = gen(hd + n_q)
+    scores = 0.3 * torch.randn(n, generator=g, device="cuda")
+    scores[0] = 18.0
+    q, c = one_number(n, hq, 1, hd, io, kv, scores, 3)
+    c.values[0].copy_(0.5 + torch.rand((n, 1, hd), generator=g, device="cuda"))
+    c.values[0][0] = 0
+    store(c)
+    q = q.expand(n_q, -1, -1).contiguous()
+    got = prefill(q, c, n - n_q, scale=0.125)[:, 0].double()
+    s = c.keys[0][:, 0, 0].double() * 0.125
+    w = (s - s[0]).exp()
+    v = c.values[0][:, 0].double()
+    l = w.cumsum(0)[-n_q:, None]
+    want = (w[:, None] * v).cumsum(0)[-n_q:] / l
+    # rows and cache of 32 bits, or f32 rows over 16 bits: sums of n positive numbers, 2^-24 each at worst
+    tol = (2.0 ** -19 + n * 2.0 ** -24) * want
+    if io != F32:
+        tol = tol + 2 * half_step(io) * want + 2 * 7.5e-5 * want
+    if kv == F16:
+        tol = tol + 2.0 ** -36 * v.cumsum(0)[-n_q:] / l
+    check(got, want, tol)
