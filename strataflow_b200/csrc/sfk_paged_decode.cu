@@ -434,9 +434,11 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 // The product has 16 rows and a CTA takes 8 heads: the other 8 rows carry what f32
 // has below 16 bits.  Rows 0-7 hold the first term of q (32-bit rows: q scaled by a
 // power of two per head, as two f16 terms) and of P, rows 8-15 the second; the two
-// halves of S and of O are added.  P reaches 2^BIAS, so that its second term keeps
-// clear of f16's smallest step; the running maximum moves when a row outgrows it by
-// 2^RAISE.
+// halves of S and of O are added.  The running maximum moves when a row outgrows it
+// by 2^RAISE; P is 2^BIAS at it.  Over f16 that is 2^11, 2^15 at most, so that P's
+// second term keeps clear of f16's smallest step; values reach 2^16 there and sums
+// stay far inside f32.  bf16 has the range of f32, values too: P is at most 1, so that
+// a finite value stays finite under it, as under the softmax's own weights.
 // Eight sequences of 131072 keys, 64 heads of 128 over 8, bf16: 645 us, 6.66 TB/s, what a
 // copy reaches (operands straight from global memory: 1190 us).  One sequence of
 // 32768, f32 rows over f16: 29.8 us, of which 20.5 are the bytes and the rest the chain
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
   using C = MmaCfg<HD, DW>;
   using Smem = MmaSmem<HD, DW>;
   constexpr int DT = DW * 32, NB = C::HDP / 64, S = C::STAGES;
-  constexpr float RAISE = 4.f, BIAS = 11.f;
+  constexpr float RAISE = 4.f, BIAS = BF16 ? -RAISE : 11.f;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;

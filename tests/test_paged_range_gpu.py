@@ -77,3 +77,47 @@ def test_prefill_dominant_key_of_zero_value(cuda, io, kv, hd, n_q, hq):
     if kv == F16:
         tol = tol + 2.0 ** -36 * v.cumsum(0)[-n_q:] / l
     check(got, want, tol)
+
+
+# ---- the largest finite values at keys that are seen ------------------------------------------------------
+@pytest.mark.parametrize("io,kv", [(F32, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("n", [40, 700, 20000])
+def test_large_finite_values_of_seen_keys(cuda, io, kv, hd, n):
+    """A weight of at most 1 times a finite value stays finite."""
+    _, c, _, _ = run_decode([n], 8, 2, hd, io, kv, 0, 0)
+    q = torch.randn((1, 8, hd), generator=gen(1), device="cuda").to(io)
+    good = decode(q, c)
+    others = [d for d in range(hd) if d != 3]
+    for j, x in ((n - 7, 1e36), (0, -1e36), (n // 2, torch.finfo(kv).max)):
+        value = c.values[0][j].clone()
+        c.values[0][j, :, 3] = x
+        store(c)
+        got = decode(q, c)
+        assert torch.equal(got[..., others], good[..., others])
+        want, tol, absv = reference(q, c.keys[0], c.values[0], [n - 1], 0, 0)
+        tol = (tol + half_step(io) * want.abs())[..., 3]
+        check(got[..., 3], want[..., 3], tol)
+        if io != F32:
+            tol = tol + (half_step(kv) + 1.5e-4) * absv[..., 3]
+        check(prefill(q, c, n - 1)[..., 3], want[..., 3], tol)
+        c.values[0][j] = value
+    store(c)
+
+
+@pytest.mark.parametrize("io,kv", [(F32, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("rise", [0.5, 2.0, 2.7, 2.9, 9.0])
+def test_decode_largest_value_at_a_score_above_the_running_maximum(cuda, io, kv, hd, rise):
+    """The largest value sits at a key that rises over all before it by less than what moves a running maximum, or by
+    more: at every place of the pages that one warp takes."""
+    n = 700
+    for j in range(0, n, 61):
+        scores = torch.zeros(n, device="cuda")
+        scores[j] = rise
+        q, c = one_number(n, 4, 1, hd, io, kv, scores, 5)
+        c.values[0].zero_()
+        c.values[0][j] = torch.finfo(kv).max
+        store(c)
+        want, tol, _ = reference(q, c.keys[0], c.values[0], [n - 1], 0, 0, 0.125)
+        check(decode(q, c, scale=0.125), want, tol + half_step(io) * want.abs())
