@@ -439,6 +439,13 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 // second term keeps clear of f16's smallest step; values reach 2^16 there and sums
 // stay far inside f32.  bf16 has the range of f32, values too: P is at most 1, so that
 // a finite value stays finite under it, as under the softmax's own weights.
+// The product's f32 sum drops what falls below its last bits, each time, towards 0: of
+// values of one sign 2.1e-4 was gone after the 2048 pages that a warp of a full batch takes
+// at 131072 keys.  So O of FOLD pages is a sum of its own, added to the kept one by f32
+// additions that round to nearest: 8 pages for 32-bit rows (4e-7 of the result, as prompts
+// have it), 512 for f16 rows (5e-5, a tenth of f16's half step).  bf16 rows keep one sum: those
+// 2.1e-4 are a twentieth of their half step, and runs of 512 pages took 673 us where one sum
+// takes 667 (eight long sequences; 32-bit rows, one sequence of 32768: 32.8, 32.0 without).
 // Eight sequences of 131072 keys, 64 heads of 128 over 8, bf16: 645 us, 6.66 TB/s, what a
 // copy reaches (operands straight from global memory: 1190 us).  One sequence of
 // 32768, f32 rows over f16: 29.8 us, of which 20.5 are the bytes and the rest the chain
@@ -509,6 +516,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
   using C = MmaCfg<HD, DW>;
   using Smem = MmaSmem<HD, DW>;
   constexpr int DT = DW * 32, NB = C::HDP / 64, S = C::STAGES;
+  constexpr int FOLD = SPLIT ? 8 : 512;  // pages (bf16: all)
   constexpr float RAISE = 4.f, BIAS = BF16 ? -RAISE : 11.f;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -611,6 +619,27 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
 #pragma unroll
   for (int i = 0; i < NB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m = -INFINITY, l = 0.f;  // of head g; l of this lane's keys
+  // The first terms' sums of whole runs of FOLD pages, in units of 2^kept_m: in registers, or, where the runs are long,
+  // in local memory (asm: so that they take no registers from the loop) from the first whole run on.
+  float kept_here[NB * 8 * 2], kept_m = -INFINITY;
+  float* kept = kept_here;
+  if constexpr (SPLIT) {
+#pragma unroll
+    for (int i = 0; i < NB * 8 * 2; ++i) kept[i] = 0.f;
+  } else if constexpr (!BF16) {
+    asm volatile("" : "+l"(kept)::"memory");
+  }
+  auto fold = [&](bool any) {  // any: there are kept sums
+    const float f = kept_m == -INFINITY ? 0.f : exp2_approx(kept_m - m);
+    kept_m = m;
+#pragma unroll
+    for (int i = 0; i < NB * 8; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        kept[2 * i + h] = SPLIT || any ? fmaf(kept[2 * i + h], f, o[i][h]) : o[i][h];
+        o[i][h] = 0.f;
+      }
+  };
   for (int k = 0; k < mine; ++k) {
     const int j0 = w.sp.page(w.i0 + warp + DW * k) * PG;
     if (!wait_slot(&sm.full[warp][k % S], (uint32_t)(k / S) & 1, p.status)) {
@@ -690,6 +719,14 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
     }
     __syncwarp();  // every lane is done with the slot
     if (k + S < mine) issue_noting(k + S);
+    if (!BF16 && k % FOLD == FOLD - 1) fold(k >= FOLD);
+  }
+  if (SPLIT || (!BF16 && mine >= FOLD)) {
+    const float f = kept_m == -INFINITY ? 0.f : exp2_approx(kept_m - m);
+#pragma unroll
+    for (int i = 0; i < NB * 8; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) o[i][h] = fmaf(kept[2 * i + h], f, o[i][h]);
   }
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);

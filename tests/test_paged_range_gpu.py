@@ -121,3 +121,68 @@ def test_decode_largest_value_at_a_score_above_the_running_maximum(cuda, io, kv,
         store(c)
         want, tol, _ = reference(q, c.keys[0], c.values[0], [n - 1], 0, 0, 0.125)
         check(decode(q, c, scale=0.125), want, tol + half_step(io) * want.abs())
+
+
+# ---- tails of one accumulator --------------------------------------------------------------------------
+def decode_as(form, q, c, table, pos):
+    """attn_decode_window with its workspace, or without one (a cluster joins the parts, or nobody)."""
+    from strataflow_b200 import lib as L
+    from strataflow_b200 import ops
+    if form == "workspace":
+        return ops.attn_decode_window(q, c.k, c.v, table, pos).view_as(q)
+    out = torch.empty_like(q)
+    n, hq, hd = q.shape
+    L.check(L.load().sfk_attn_decode_window(ops._ROW_TYPES[q.dtype], q.data_ptr(), hq * hd, ops._KV_TYPES[c.k.dtype],
+                                            c.k.data_ptr(), c.v.data_ptr(), c.k.shape[0], table.data_ptr(),
+                                            table.shape[1], pos.data_ptr(), n, hq, c.kvh, hd, 0.0, 0, 0, out.data_ptr(),
+                                            None, 0, None, torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+# "many": the same sequence as many times as it takes to give each (sequence, kv head) one CTA
+FORMS = [("workspace", 1), ("cluster", 1), ("many", 300)]
+
+
+@pytest.mark.parametrize("form,copies", FORMS)
+@pytest.mark.parametrize("kv", [F32, F16, BF16])
+def test_decode_of_32_bit_rows_has_no_drift(cuda, form, copies, kv):
+    """Values of one sign at 131072 keys: sums that only grow.  A sum of c numbers, each addition rounded to nearest:
+    steps of 2^-23 of the partial sum at most, 0.72 of that on average, rms 0.72 * 2^-23 / 12^(1/2) (c / 3)^(1/2) of the
+    result.  A warp of a sequence's only CTA adds a quarter of the keys: 2.6e-6, and four of them meet: 1.3e-6 an
+    element, of which 2^-18 is three times.  The gain is a mean over 1024 such elements, with the error of the weights'
+    sum (32 sums of an eighth of these: 1.6e-7): below 2^-20.  Additions that truncate would lose
+    0.72 * 2^-24 c / 2 with c the products on one accumulator."""
+    n, hd = 131072, 128
+    c = Cache([n], 1, hd, kv, 14)
+    c.values[0].copy_(0.5 + torch.rand((n, 1, hd), generator=gen(15), device="cuda"))
+    store(c)
+    copies = min(copies, 600) * 2
+    q = torch.randn((copies, 4, hd), generator=gen(16), device="cuda") * 0.25
+    table, pos = c.table.expand(copies, -1).contiguous(), torch.full((copies,), n - 1, dtype=torch.int32, device="cuda")
+    got = decode_as(form, q, c, table, pos)[:2].double()
+    want = reference(q[:2], c.keys[0], c.values[0], [n - 1] * 2, 0, 0)[0]
+    gain = float((got * want).sum() / (want * want).sum()) - 1
+    assert abs(gain) < 2.0 ** -20, gain
+    assert float((got - want).norm() / want.norm()) < 2.0 ** -18
+
+
+@pytest.mark.parametrize("form,copies", FORMS)
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_decode_of_16_bit_rows_has_no_drift(cuda, form, copies, kv, hd):
+    """The same of 16-bit rows, each dim in a scale of its own, so that their roundings are independent: the gain is
+    off by the mean of hd of them, 0.42 half_step / hd^(1/2) as a root of squares, four of these 0.21 half_step at 64,
+    and by what a sum may lose: a quarter of half a step for both."""
+    n = 131072
+    c = Cache([n], 1, hd, kv, 14)
+    scales = 2.0 ** (torch.arange(hd, device="cuda") / hd)
+    c.values[0].copy_((0.5 + torch.rand((n, 1, hd), generator=gen(15), device="cuda")) * scales)
+    store(c)
+    copies = min(copies, 600) * 2
+    q = (torch.randn((copies, 4, hd), generator=gen(16), device="cuda") * 0.25).to(kv)
+    table, pos = c.table.expand(copies, -1).contiguous(), torch.full((copies,), n - 1, dtype=torch.int32, device="cuda")
+    got = decode_as(form, q, c, table, pos)[:2].double()
+    want = reference(q[:2], c.keys[0], c.values[0], [n - 1] * 2, 0, 0)[0]
+    gain = float((got * want).sum() / (want * want).sum()) - 1
+    assert abs(gain) < half_step(kv) / 4, gain
+    assert float((got - want).norm() / want.norm()) < half_step(kv)
