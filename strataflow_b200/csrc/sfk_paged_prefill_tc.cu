@@ -41,6 +41,13 @@
 // above 30000 others: 0.95 of the tail lost): P is 2^11 at m, 2^15 at most, and a
 // weight is held to half a step of f16 or 2^-36 of the largest.
 //
+// The accumulator of a product drops what falls below its last bits, each time, towards
+// 0: 8.3e-4 of values of one sign were gone after 131072 keys, more than half a step of
+// f16.  So f16 rows start O anew every 10240 keys and keep the sum in local memory, added
+// to the nearest (6.7e-5; 2048 tokens at 30000 keys, 32 heads of 128: 875 us with and
+// without, heads of 64: 858 and 832).  bf16 rows keep one accumulator: those 8.3e-4 are a
+// fifth of their half step, and a second loop around the tiles took 2 % there.
+//
 // 32-bit rows over an f16 cache (SPLIT): q, scaled by a power of two per row,
 // is the sum of two f16 numbers and so is each P (22 bits), and each product
 // is two.  P's range is that of f16 rows, so that its second part too stays above
@@ -331,6 +338,8 @@ __global__ void __launch_bounds__(TT, 1)
   using C = Cfg<HD, SPLIT>;
   constexpr bool BF16 = std::is_same<KV, __nv_bfloat16>::value;
   constexpr int HDP = C::HDP, NS = C::NS, TK = C::TK, PPT = C::PPT;
+  constexpr bool RUNS = !SPLIT && !BF16;               // O is the sum of several accumulators
+  constexpr int RUN = RUNS ? 128 * 80 / TK : 1 << 30;  // key tiles of one
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = base;                   // [tile][term][half][128 rows][128 B]
@@ -568,103 +577,130 @@ __global__ void __launch_bounds__(TT, 1)
       };
       if (!adds) {
         float m = -INFINITY, l = 0.f;  // m in scaled log2 units
-        for (int n = 0; n < nk; ++n) {
-          if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
-          fence_after();
-          // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
-          const int e0 = (n_first + n) * PPT;
-          const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
-                             (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
-          if (!inner) {
-            // what the row does not see becomes -inf, in place
+        // O of whole runs of RUN key tiles, in units of 2^kept_m: in local memory, touched once a run
+        volatile float kept[RUNS ? HDP : 1];
+        float kept_m = -INFINITY;
+        auto fold = [&](bool any) {  // any: there are kept sums.  O is complete, and 0 from here on.
+          const float f = kept_m == -INFINITY ? 0.f : exp2_approx(kept_m - m);
+          kept_m = m;
 #pragma unroll 1
-            for (int g = 0; g < PPT; ++g) {
-              const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
-              if (jb + PG - 1 <= t_lo && (p.window == 0 || jb > t_hi - p.window)) continue;  // every row sees the page
-              const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
-              float s[16];
-              tmem_ld16(ts + g * PG, s);
+          for (int d = 0; d < HDP; d += 16) {
+            float o[16];
+            tmem_ld16(to + d, o);
 #pragma unroll
-              for (int k = 0; k < PG; ++k) s[k] = k <= hi && (k > lo || k < sk) ? s[k] : -INFINITY;
-              tmem_st16(ts + g * PG, s);
+            for (int k = 0; k < 16; ++k) {
+              kept[d + k] = any ? fmaf(kept[d + k], f, o[k]) : o[k];
+              o[k] = 0.f;
             }
-            tmem_st_wait();
+            tmem_st16(to + d, o);
           }
-          float s[TK];
-          tmem_ld(ts, s);
-          if (n + 1 < nk) done(&c->s_free[w]);  // the next Q K^T may begin
-          float m4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int k = 4; k < TK; k += 4)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m4[i] = max_nan(m4[i], s[k + i]);
-          float mx = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
-          // O is complete and P may be written again (mostly long since)
-          if (n > 0) {
-            if (!(ok = wait_warp(&c->pv_done[w], (n - 1) & 1, c))) break;
-            fence_after();
-          }
-          mx *= scale;
-          float f = 1.f;
-          if (__any_sync(0xffffffffu, !(mx <= m + RAISE))) {
-            // a row that saw a score of NaN or +inf is NaN, by its m: the polynomial below does not carry these on
-            const float mn = max_nan(mx, m) < INFINITY ? fmaxf(mx, m) : NAN;
-            f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
-            m = mn;
-            l *= f;
-            if (!SPLIT && n > 0) {
-#pragma unroll 1
-              for (int d = 0; d < HDP; d += 16) {
-                float o[16];
-                tmem_ld16(to + d, o);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] *= f;
-                tmem_st16(to + d, o);
-              }
-            }
-          }
-          if constexpr (SPLIT) {  // the other warpgroup rescales
-            factor[n % 4 * TM + row] = f;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&c->f_full[n % 4]);
-          }
-          const float neg = BIAS - (m == -INFINITY ? 0.f : m);
-          const uint64_t scale2 = both(scale), neg2 = both(neg), up2 = both(neg + POLY_UP);
-          uint64_t sum2 = 0;
-#pragma unroll
-          for (int b = 0; b < PPT; ++b) {  // 16 keys: 8 columns of P
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const bool poly = (k * 3) % 8 < C::POLY_OF_8;
-              const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, BF16 && poly ? up2 : neg2);
-              float x, y;
-              if (poly) {
-                exp2_poly<BF16>(x2, x, y);
-              } else {
-                unpair(x2, x, y);
-                x = exp2_approx(x);
-                y = exp2_approx(y);
-              }
-              sum2 = add2(sum2, pair(x, y));
-              hi[k] = pack2<BF16>(x, y);
-              if constexpr (SPLIT) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-                lo[k] = pack2<false>(x - f.x, y - f.y);
-              }
-            }
-            tmem_st8(tp + b * 8, hi);
-            if constexpr (SPLIT) tmem_st8(tp + TK / 2 + b * 8, lo);
-            if ((b + 1) * PG == C::FIRST) {  // the product of these keys may begin
-              tmem_st_wait();
-              done(&c->p_full[w][0]);
-            }
-          }
-          float l0, l1;
-          unpair(sum2, l0, l1);
-          l += l0 + l1;
           tmem_st_wait();
-          done(&c->p_full[w][1]);
+        };
+        for (int n0 = 0; n0 < (RUNS ? nk : 1) && ok; n0 += RUN) {
+          if (RUNS && n0 > 0) {
+            if (!(ok = wait_warp(&c->pv_done[w], (n0 - 1) & 1, c))) break;
+            fence_after();
+            fold(n0 > RUN);
+          }
+          const int n1 = RUNS ? min(n0 + RUN, nk) : nk;
+          for (int n = n0; n < n1; ++n) {
+            if (!(ok = wait_warp(&c->s_full[w], n & 1, c))) break;
+            fence_after();
+            // every key of the tile seen by every row: whole pages, none past the first row's position, all in the last row's window
+            const int e0 = (n_first + n) * PPT;
+            const bool inner = e0 >= sp.sink && e0 + PPT <= sp.n && sp.page(e0 + PPT - 1) * PG + PG - 1 <= t_lo &&
+                               (p.window == 0 || sp.page(e0) * PG > t_hi - p.window);
+            if (!inner) {
+              // what the row does not see becomes -inf, in place
+#pragma unroll 1
+              for (int g = 0; g < PPT; ++g) {
+                const int jb = e0 + g < sp.n ? sp.page(e0 + g) * PG : 0x7fffff00;
+                if (jb + PG - 1 <= t_lo && (p.window == 0 || jb > t_hi - p.window)) continue;  // every row sees the page
+                const int hi = pos - jb, lo = p.window ? hi - p.window : -1, sk = p.window ? p.n_sink - jb : 0;
+                float s[16];
+                tmem_ld16(ts + g * PG, s);
+#pragma unroll
+                for (int k = 0; k < PG; ++k) s[k] = k <= hi && (k > lo || k < sk) ? s[k] : -INFINITY;
+                tmem_st16(ts + g * PG, s);
+              }
+              tmem_st_wait();
+            }
+            float s[TK];
+            tmem_ld(ts, s);
+            if (n + 1 < nk) done(&c->s_free[w]);  // the next Q K^T may begin
+            float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int k = 4; k < TK; k += 4)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) m4[i] = max_nan(m4[i], s[k + i]);
+            float mx = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
+            // O is complete and P may be written again (mostly long since)
+            if (n > 0) {
+              if (!(ok = wait_warp(&c->pv_done[w], (n - 1) & 1, c))) break;
+              fence_after();
+            }
+            mx *= scale;
+            float f = 1.f;
+            if (__any_sync(0xffffffffu, !(mx <= m + RAISE))) {
+              // a row that saw a score of NaN or +inf is NaN, by its m: the polynomial below does not carry these on
+              const float mn = max_nan(mx, m) < INFINITY ? fmaxf(mx, m) : NAN;
+              f = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+              m = mn;
+              l *= f;
+              if (!SPLIT && n > 0) {
+#pragma unroll 1
+                for (int d = 0; d < HDP; d += 16) {
+                  float o[16];
+                  tmem_ld16(to + d, o);
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) o[k] *= f;
+                  tmem_st16(to + d, o);
+                }
+              }
+            }
+            if constexpr (SPLIT) {  // the other warpgroup rescales
+              factor[n % 4 * TM + row] = f;
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&c->f_full[n % 4]);
+            }
+            const float neg = BIAS - (m == -INFINITY ? 0.f : m);
+            const uint64_t scale2 = both(scale), neg2 = both(neg), up2 = both(neg + POLY_UP);
+            uint64_t sum2 = 0;
+#pragma unroll
+            for (int b = 0; b < PPT; ++b) {  // 16 keys: 8 columns of P
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const bool poly = (k * 3) % 8 < C::POLY_OF_8;
+                const uint64_t x2 = fma2(pair(s[b * 16 + 2 * k], s[b * 16 + 2 * k + 1]), scale2, BF16 && poly ? up2 : neg2);
+                float x, y;
+                if (poly) {
+                  exp2_poly<BF16>(x2, x, y);
+                } else {
+                  unpair(x2, x, y);
+                  x = exp2_approx(x);
+                  y = exp2_approx(y);
+                }
+                sum2 = add2(sum2, pair(x, y));
+                hi[k] = pack2<BF16>(x, y);
+                if constexpr (SPLIT) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                  lo[k] = pack2<false>(x - f.x, y - f.y);
+                }
+              }
+              tmem_st8(tp + b * 8, hi);
+              if constexpr (SPLIT) tmem_st8(tp + TK / 2 + b * 8, lo);
+              if ((b + 1) * PG == C::FIRST) {  // the product of these keys may begin
+                tmem_st_wait();
+                done(&c->p_full[w][0]);
+              }
+            }
+            float l0, l1;
+            unpair(sum2, l0, l1);
+            l += l0 + l1;
+            tmem_st_wait();
+            done(&c->p_full[w][1]);
+          }
         }
         if constexpr (SPLIT) {
           last[row] = make_float2(m, l);
@@ -676,7 +712,17 @@ __global__ void __launch_bounds__(TT, 1)
             fence_after();
           }
           if (parts > 1) asm volatile("bar.sync 1, %0;" ::"r"(n_tiles * TM) : "memory");  // both row tiles are through
-          if (ok) finish([&](int d, float(&o)[32]) { tmem_ld32(to + d, o); }, m, l);
+          if (ok)
+            finish(
+                [&](int d, float(&o)[32]) {
+                  tmem_ld32(to + d, o);
+                  if (RUNS && nk > RUN) {
+                    const float f = kept_m == -INFINITY ? 0.f : exp2_approx(kept_m - m);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = fmaf(kept[d + k], f, o[k]);
+                  }
+                },
+                m, l);
         }
       } else if constexpr (SPLIT) {
         // Each tile's O is a product of its own, added here: the tensor core's f32 accumulator drops what falls below
