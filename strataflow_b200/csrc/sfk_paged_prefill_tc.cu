@@ -523,7 +523,8 @@ __global__ void __launch_bounds__(TT, 1)
         constexpr int ES = SPLIT ? 4 : 2, CH = HD * ES / 16;  // bytes of an output element, chunks of a row
         constexpr int X = CH < 8 ? CH - 1 : 7;
         uint8_t* rows = qs + w * NS * C::QTILE + wrow % TM * (HD * ES);
-        const float inv = 1.0f / l;
+        // a row whose every seen score is -inf has no weights: NaN, where the polynomial's 2^-126 would leave a sum
+        const float inv = 1.0f / (m == -INFINITY ? 0.f : l);
         bool finite = true;
 #pragma unroll(SPLIT ? HD / 32 : 1)
         for (int d = 0; d < HD; d += 32) {

@@ -207,3 +207,29 @@ def test_prefill_of_16_bit_rows_has_no_drift(cuda, kv, hd, n_q):
         gain = float((got[i:i + 1].double() * want).sum() / (want * want).sum()) - 1
         assert abs(gain) < 0.41 * half_step(kv), gain
         assert float((got[i:i + 1].double() - want).norm() / want.norm()) < half_step(kv)
+
+
+# ---- no weight at all ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("n", [40, 700, 9000])
+def test_rows_of_scores_of_minus_infinity_alone(cuda, io, kv, hd, n):
+    """A row all of whose seen keys score -inf has no weights: NaN; later rows are as if those keys were not there."""
+    hidden = 21
+    c = Cache([n], 2, hd, kv, 9)
+    q = torch.randn((n, 4, hd), generator=gen(10), device="cuda").to(io)
+    q[..., 0] = q[..., 0].abs() + 1
+    c.keys[0][:hidden] = 0
+    c.keys[0][:hidden, :, 0] = -math.inf
+    store(c)
+    got = prefill(q, c, 0)
+    assert got[:hidden].isnan().all()
+    rows = sorted({hidden, hidden + 1, n - 1})
+    want, tol, absv = reference(q[rows], c.keys[0][hidden:], c.values[0][hidden:], [r - hidden for r in rows], 0, 0)
+    if io != F32:
+        tol = tol + half_step(io) * want.abs() + (half_step(kv) + 1.5e-4) * absv
+    check(got[rows], want, tol)
+    assert got[hidden:].isfinite().all()
+    from strataflow_b200 import ops
+    pos = torch.tensor([hidden - 1], dtype=torch.int32, device="cuda")
+    assert ops.attn_decode_window(q[hidden - 1:hidden], c.k, c.v, c.table, pos).isnan().all()
