@@ -489,6 +489,52 @@ __device__ __forceinline__ float add_terms(float first, float second) {
   return fabsf(first) < INFINITY ? first + second : first;
 }
 
+// One query head's part of one warp again, in f32, key by key: o to `out`, (m, l) returned, weights `one` at m.  For a
+// part that came out as NaN over an f16 cache: a weight (or a number of q) whose first term rounds to 0 makes NaN of an
+// infinite value (or key), where the formula has an infinite output (or a weight of 0).
+template <class KV, int HD, int DW>
+__device__ __noinline__ float2 recompute_part(const WindowAttnParams& p, const Work w, int row, float one, float* out) {
+  constexpr int E = HD / 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, key = lane % PG, half = lane / PG * (HD / 2);
+  const int64_t q0 = w.seq * p.q_stride + (int64_t)(w.head0 + row) * HD + half;
+  float m = -INFINITY, l = 0.f, o[E] = {};
+  for (int i = w.i0 + warp; i < w.i1; i += DW) {
+    const int id = page_id(p, w, i);
+    if (id < 0) continue;  // the same for all lanes
+    const int64_t page = ((int64_t)id * p.n_head_kv + w.hk) * PG * HD;
+    const KV* k = static_cast<const KV*>(p.k_pages) + page + key * HD + half;
+    const KV* v = static_cast<const KV*>(p.v_pages) + page + lane * E;
+    float s = 0.f;
+#pragma unroll 8
+    for (int d = 0; d < HD / 2; ++d) s = fmaf(load_elem(p.q, q0 + d, p.io), to_f32<KV>(k[d]), s);
+    s += __shfl_xor_sync(0xffffffffu, s, PG);
+    const bool see = key_seen(w.sp.page(i) * PG + key, w.pos, p.window, p.n_sink);
+    s = see ? s * p.scale_log2 : -INFINITY;
+    float mx = s;
+#pragma unroll
+    for (int d = 1; d < PG; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    mx = fmaxf(mx, m);
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    const float f = exp2_approx(m - ms), x = exp2_approx(s - ms);
+    m = mx;
+    l = l * f + x;  // of this lane's key
+    const unsigned seen = __ballot_sync(0xffffffffu, see);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= f;
+    for (int j = 0; j < PG; ++j) {
+      const float xj = __shfl_sync(0xffffffffu, x, j);
+      if (!(seen >> j & 1)) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(xj, to_f32<KV>(v[j * HD + e]), o[e]);
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < PG; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[lane * E + e] = o[e] * one;
+  return make_float2(m, l * one);
+}
+
 template <int HD, int DW>
 struct MmaCfg {
   static constexpr int HDP = HD < 64 ? 64 : HD;    // head width in a slot (the copy fills with zeros)
@@ -743,6 +789,23 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
       if (d < HD) sm.join.o[warp][g][d] = add_terms(o[b * 8 + e][0], o[b * 8 + e][2]);
       if (d + 8 < HD) sm.join.o[warp][g][d + 8] = add_terms(o[b * 8 + e][1], o[b * 8 + e][3]);
     }
+  if constexpr (!BF16) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < NB * 8; ++i) nan = nan || o[i][0] != o[i][0] || o[i][1] != o[i][1];
+    // rows of one term of q: a sum of weights that is not finite is the formula's
+    unsigned again = __ballot_sync(0xffffffffu, nan && g < w.n_rows && (SPLIT || l < INFINITY));
+    while (again) {
+      const int r = (__ffs(again) - 1) / 4;
+      again &= ~(0xfu << (4 * r));
+      __syncwarp();
+      const float2 ml = recompute_part<KV, HD, DW>(p, w, r, 1 << (int)BIAS, sm.join.o[warp][r]);
+      if (lane == 0) {
+        sm.join.m[warp][r] = ml.x;
+        sm.join.l[warp][r] = ml.y;
+      }
+    }
+  }
   join_and_store(sm.join, p, w.seq, w.head0, w.n_rows, w.pos >= 0);
 }
 

@@ -233,3 +233,57 @@ def test_rows_of_scores_of_minus_infinity_alone(cuda, io, kv, hd, n):
     from strataflow_b200 import ops
     pos = torch.tensor([hidden - 1], dtype=torch.int32, device="cuda")
     assert ops.attn_decode_window(q[hidden - 1:hidden], c.k, c.v, c.table, pos).isnan().all()
+
+
+# ---- infinite keys and values of tiny weight --------------------------------------------------------------
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("n", [40, 700, 20000])
+@pytest.mark.parametrize("below", [10.0, 20.0, 40.0, 80.0])
+def test_infinite_value_of_a_tiny_weight(cuda, io, kv, hd, n, below):
+    """e^-below of the row's largest weight times an infinite value is infinite, for single tokens and for prompts; the
+    other kv head and the other dims are as they were.  (Down to e^-80 = 2^-116: from 2^-126 on a weight is 0.)"""
+    from strataflow_b200 import ops
+    scores = torch.zeros(n, device="cuda")
+    j = n // 2 + 3
+    scores[j] = -below
+    q, c = one_number(n, 8, 2, hd, io, kv, scores, 7)
+    others = [d for d in range(hd) if d != 3]
+    start = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+
+    def prompt():
+        return ops.attn_prefill_window(q, c.k, c.v, c.table, start, start[1:] * n, scale=0.125).view_as(q)
+
+    for f in (lambda: decode(q, c, scale=0.125), prompt):
+        good = f()
+        for x in (math.inf, -math.inf, math.nan):
+            value = c.v[c.table[0, j // PG], 0, j % PG, 3].clone()
+            c.v[c.table[0, j // PG], 0, j % PG, 3] = x
+            got = f()
+            c.v[c.table[0, j // PG], 0, j % PG, 3] = value
+            want = torch.full((4,), x, device="cuda", dtype=io)
+            assert torch.allclose(got[0, :4, 3], want, equal_nan=True)
+            assert torch.equal(got[0, 4:], good[0, 4:])
+            w, tol, absv = reference(q, c.keys[0], c.values[0], [n - 1], 0, 0, 0.125)
+            if io != F32:
+                tol = tol + half_step(io) * w.abs() + (half_step(kv) + 1.5e-4) * absv
+            check(got[..., others], w[..., others], tol.expand_as(w)[..., others])
+
+
+@pytest.mark.parametrize("io,kv", [(F32, F32), (F32, F16), (F32, BF16)])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("n", [40, 700, 20000])
+def test_infinite_key_times_a_tiny_query(cuda, io, kv, hd, n):
+    """A number of q 2^-30 below the row's largest times an infinite key: -inf takes the key out, +inf makes the row NaN."""
+    _, c, _, _ = run_decode([n], 8, 2, hd, io, kv, 0, 0)
+    q = torch.randn((1, 8, hd), generator=gen(1), device="cuda")
+    q[..., 0] = torch.tensor([1.0, -1.0], device="cuda").repeat(4) * 2.0 ** -30
+    j = n // 2 + 3
+    kept = [i for i in range(n) if i != j]
+    want, tol, _ = reference(q, c.keys[0][kept], c.values[0][kept], [n - 2], 0, 0)
+    c.keys[0][j] = 0
+    c.keys[0][j, :, 0] = math.inf
+    store(c)
+    for got in (decode(q, c), prefill(q, c, n - 1)):
+        assert got[:, 0::2].isnan().all()
+        check(got[:, 1::2], want[:, 1::2], tol[:, 1::2])
