@@ -552,7 +552,8 @@ SFK_API sfk_status sfk_qk_norm_rope_append(
  * j > p - window or j < n_sink.  scale 0: 1 / sqrt(head_dim).  A negative
  * position is a padding row and gives zeros.  head_dim 32, 64, 128 or 256; any
  * number of query heads per kv head; 16-bit rows need a cache of their own
- * type, f32 rows take any.  out: [n_seq][n_head * head_dim].
+ * type, f32 rows take any.  out: [n_seq][n_head * head_dim]; q itself where
+ * q's rows are contiguous, otherwise apart from them.
  * dev_workspace (optional, 16-byte aligned device memory) belongs to the call
  * until its work is done and holds nothing between calls; with less than
  * sfk_attn_decode_window_workspace bytes, or none, a small batch over a long
@@ -575,7 +576,7 @@ SFK_API size_t sfk_attn_decode_window_workspace(int32_t n_seq, int32_t n_head, i
  * (kv_len device), and token i of them sits at position kv_len[s] - n_q + i.
  * A token whose position is negative sees nothing and gives zeros; rows of q
  * outside every sequence are neither read nor written.
- * out: [n_tok][n_head * head_dim], apart from q. */
+ * out: [n_tok][n_head * head_dim], apart from q's rows. */
 SFK_API sfk_status sfk_attn_prefill_window(int32_t io_type, const void *dev_q, int64_t q_stride, int32_t n_tok,
                                            int32_t kv_type, const void *dev_k_pages, const void *dev_v_pages,
                                            int32_t n_pages, const int32_t *dev_page_table, int32_t max_pages,

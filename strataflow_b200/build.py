@@ -30,7 +30,7 @@ SOURCES = ["sfk_kernels.cu", "sfk_mega.cu", "sfk_tc.cu", "sfk_prefill.cu", "sfk_
            "sfk_paged_prefill_tc.cu", "sfk_paged_api.cu",
            "sfk_strata.cpp", "sfk_tier.cpp"]
 HEADERS = ["sfk_device.cuh", "sfk_act.cuh", "sfk_dequant.cuh", "sfk_kernels.cuh", "sfk_route.cuh", "sfk_mega.cuh",
-           "sfk_tc.cuh", "sfk_prefill.cuh", "sfk_sample.cuh", "sfk_paged.cuh", "sfk_paged_map.cuh", "sfk_tier.h"]
+           "sfk_tc.cuh", "sfk_prefill.cuh", "sfk_sample.cuh", "sfk_paged.cuh", "sfk_paged_map.cuh", "sfk_rows.h", "sfk_tier.h"]
 
 
 def nvcc() -> str:

@@ -10,6 +10,7 @@
 #include "../../include/sfk.h"
 #include "sfk_kernels.cuh"
 #include "sfk_paged.cuh"
+#include "sfk_rows.h"
 
 using namespace sfk;
 
@@ -38,6 +39,10 @@ int kv_elem(int t) { return t == SFK_KV_F32 ? EL_F32 : t == SFK_KV_F16 ? EL_F16 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // rows of `stride` elements from p keep 16-byte alignment
 bool vec_rows(const void* p, int64_t stride, int elem) { return aligned16(p) && stride * elem_size(elem) % 16 == 0; }
+
+Rows rows_of(const void* at, int64_t stride, int64_t width, int64_t n, int elem) {
+  return {at, stride * elem_size(elem), width * elem_size(elem), n};
+}
 
 int current_sms() {
   static int cached[64];  // multiprocessors of each device; every writer writes the same number
@@ -172,6 +177,10 @@ sfk_status sfk_attn_decode_window(int32_t io_type, const void* q, int64_t q_stri
     return s;
   if (!positions) BAD("%s: null pointer", who);
   if (!aligned16(workspace)) BAD("%s: the workspace starts on a 16-byte boundary", who);
+  // in place a CTA reads the heads that it writes, and no others; else one sequence's output would be another's query
+  const int64_t width = (int64_t)n_head * hd;
+  const Rows qr = rows_of(q, q_stride, width, n_seq, a.io), outr = rows_of(out, width, width, n_seq, a.io);
+  if (!same_rows(qr, outr) && rows_meet(qr, outr)) BAD("%s: out overlaps q (only its own rows, contiguous, may be)", who);
   a.partial = static_cast<float*>(workspace);
   a.ws_bytes = workspace ? workspace_bytes : 0;
   a.pos = positions;
@@ -211,7 +220,10 @@ sfk_status sfk_attn_prefill_window(int32_t io_type, const void* q, int64_t q_str
   if (!q_start || !kv_len) BAD("%s: null pointer", who);
   if (n_head_kv > 65535 || (int64_t)n_tok * (n_head / n_head_kv) > (1ll << 30))
     BAD("%s: %d tokens of %d heads in one call", who, n_tok, n_head);
-  if (out == q) BAD("%s: out is q", who);  // a row may be read again after others of its tile are written
+  // a row may be read again after others of its tile are written
+  const int64_t width = (int64_t)n_head * hd;
+  if (rows_meet(rows_of(q, q_stride, width, n_tok, a.io), rows_of(out, width, width, n_tok, a.io)))
+    BAD("%s: out is q, or overlaps it", who);
   a.q_start = q_start;
   a.kv_len = kv_len;
   a.n_seq = n_seq;

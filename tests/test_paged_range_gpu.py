@@ -287,3 +287,33 @@ def test_infinite_key_times_a_tiny_query(cuda, io, kv, hd, n):
     for got in (decode(q, c), prefill(q, c, n - 1)):
         assert got[:, 0::2].isnan().all()
         check(got[:, 1::2], want[:, 1::2], tol[:, 1::2])
+
+
+# ---- out and q in one buffer --------------------------------------------------------------------------------
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("n,n_seq", [(40, 1), (700, 3), (20000, 1), (300, 40)])
+def test_decode_in_place_and_between_rows(cuda, io, kv, n, n_seq):
+    """out = q, out in the gap between q's rows, out right behind and right before q's rows: the bits of an out of its
+    own.  out over a wider q is refused."""
+    from strataflow_b200 import lib as L
+    hq, hd = 8, 64
+    c = Cache([n] * n_seq, 2, hd, kv, 1)
+    q = torch.randn((n_seq, hq, hd), generator=gen(2), device="cuda").to(io)
+    want = decode(q, c)
+    mine = q.clone()
+    decode(mine, c, out=mine.view(n_seq, hq * hd))
+    assert torch.equal(mine, want)
+    buf = torch.zeros((n_seq, (n_seq + 1) * hq * hd), dtype=io, device="cuda")
+    wide = buf[:, :hq * hd].unflatten(1, (hq, hd))
+    wide.copy_(q)
+    decode(wide, c, out=buf[0, hq * hd:].view(n_seq, hq * hd))
+    assert torch.equal(buf[0, hq * hd:].view_as(want), want) and torch.equal(wide, q)
+    flat = torch.zeros((3 * n_seq, hq * hd), dtype=io, device="cuda")
+    own = flat[n_seq:2 * n_seq].unflatten(1, (hq, hd))
+    own.copy_(q)
+    for out in (flat[:n_seq], flat[2 * n_seq:]):
+        decode(own, c, out=out)
+        assert torch.equal(out.view_as(want), want) and torch.equal(own, q)
+    if n_seq > 1:
+        with pytest.raises(L.SfkError, match="overlaps"):
+            decode(wide, c, out=buf.view(-1)[:n_seq * hq * hd].view(n_seq, -1))
