@@ -537,7 +537,8 @@ SFK_API sfk_status sfk_attn_decode_paged(const float *dev_q, const void *dev_k_p
  *             sequence t).  pos[t] < 0: a padding row, nothing of it is
  *             written.  A slot is given at most once in a call.
  * head_dim is a multiple of 8 up to 256; any io_type with any kv_type, rounded
- * once.  q_out may be q itself (same stride). */
+ * once.  q_out may be q itself (same stride), and is otherwise apart from the
+ * rows of q, k and v. */
 SFK_API sfk_status sfk_qk_norm_rope_append(
     int32_t io_type, const void *dev_q, int64_t q_stride, const void *dev_k, int64_t k_stride, const void *dev_v,
     int64_t v_stride, int32_t n_tok, int32_t n_head, int32_t n_head_kv, int32_t head_dim, const float *dev_q_norm,

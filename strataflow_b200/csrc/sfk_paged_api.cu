@@ -126,6 +126,11 @@ sfk_status sfk_qk_norm_rope_append(int32_t io_type, const void* q, int64_t q_str
   if (!aligned16(kp) || !aligned16(vp)) BAD("%s: page pools start on 16-byte boundaries", who);
   const int64_t nq = (int64_t)n_head * hd, nk = (int64_t)n_head_kv * hd;
   if (q_stride < nq || k_stride < nk || v_stride < nk || q_out_stride < nq) BAD("%s: strides below a token's row", who);
+  // in place a warp has read the row that it writes; a row of another token, or of k or v, may still be waited for
+  const Rows qr = rows_of(q, q_stride, nq, n_tok, io), outr = rows_of(q_out, q_out_stride, nq, n_tok, io);
+  if (!same_rows(qr, outr) && rows_meet(qr, outr)) BAD("%s: q_out overlaps q (only q itself, in q's stride, may be)", who);
+  if (rows_meet(rows_of(k, k_stride, nk, n_tok, io), outr) || rows_meet(rows_of(v, v_stride, nk, n_tok, io), outr))
+    BAD("%s: q_out overlaps k or v", who);
   AppendParams p{};
   p.q = q;
   p.k = k;

@@ -317,3 +317,33 @@ def test_decode_in_place_and_between_rows(cuda, io, kv, n, n_seq):
     if n_seq > 1:
         with pytest.raises(L.SfkError, match="overlaps"):
             decode(wide, c, out=buf.view(-1)[:n_seq * hq * hd].view(n_seq, -1))
+
+
+@pytest.mark.parametrize("io", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [1, 5, 3000])
+def test_append_in_place_of_a_packed_row(cuda, io, n):
+    """q_out = q inside packed rows, its k and v beside it: the bits of an out of its own; k and v as they were.  q_out
+    over k, or over q in another stride, is refused."""
+    from strataflow_b200 import lib as L
+    from strataflow_b200 import ops
+    hq, hkv, hd = 8, 2, 64
+    x = torch.randn((n, hq + 2 * hkv, hd), generator=gen(3), device="cuda").to(io)
+    y = x.clone()
+    pages = (n + PG - 1) // PG
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+
+    def run(rows, out):
+        pools = torch.zeros((2, pages, hkv, PG, hd), dtype=io, device="cuda")
+        got = ops.qk_norm_rope_append(rows[:, :hq], rows[:, hq:hq + hkv], rows[:, hq + hkv:], pools[0], pools[1], table, pos,
+                                      seq=torch.zeros_like(pos), freqs=ops.rope_freqs(hd), neox=True, out=out)
+        return got, pools
+
+    want, pools = run(x, None)
+    got, mine = run(y, y[:, :hq])
+    assert torch.equal(got, want) and torch.equal(mine, pools) and torch.equal(y[:, hq:], x[:, hq:])
+    for bad in (x[:, 1:hq + 1], x[:, 2 * hkv:], x.view(-1)[:n * hq * hd].view(n, hq, hd)):
+        if n == 1 and bad.data_ptr() == x.data_ptr():
+            continue
+        with pytest.raises(L.SfkError, match="overlaps"):
+            run(x, bad)

@@ -45,3 +45,16 @@ def test_decode_refuses_an_out_that_overlaps_q(sfk, kw):  # noqa: F811
 def test_prefill_refuses_an_out_that_overlaps_q(sfk, kw):  # noqa: F811
     assert call(sfk, "sfk_attn_prefill_window", PREFILL, **kw) == L.SFK_ERR_INVALID_ARGUMENT
     assert b"overlaps it" in sfk.sfk_last_error()
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(outs=8 * 64 + 8), b"overlaps q"), (dict(out=X + 4), b"overlaps q"), (dict(out=X + ROW), b"overlaps q"),
+    (dict(out=X - 3 * ROW + 4, outs=8 * 64), b"overlaps q"), (dict(qs=12 * 64, outs=8 * 64), b"overlaps q"),
+    (dict(k=X + ROW - 4, v=X + (1 << 16)), b"overlaps k or v"),
+    (dict(k=X + (1 << 16), v=X + 2 * ROW, vs=4 * 64), b"overlaps k or v"),
+    (dict(n=1, k=X + ROW - 4, v=X + (1 << 16)), b"overlaps k or v"),
+])
+def test_append_refuses_a_q_out_that_overlaps_other_rows(sfk, kw, why):  # noqa: F811
+    kw = {"k": X + (1 << 16), "v": X + (1 << 17), **kw}
+    assert call(sfk, "sfk_qk_norm_rope_append", APPEND, **kw) == L.SFK_ERR_INVALID_ARGUMENT
+    assert why in sfk.sfk_last_error()
