@@ -519,7 +519,9 @@ SFK_API sfk_status sfk_attn_decode_paged(const float *dev_q, const void *dev_k_p
  *     dereferenced; it stores a code there, and sfk_device_status (which waits
  *     for the stream) turns the code into SFK_ERR_RUNTIME and clears the word.
  *     What the call then gives for that sequence is not specified; the others
- *     are not touched by it.
+ *     are not touched by it.  The attention kernels' waits for their own copies
+ *     and products are bounded (about a second); one that runs out stores a
+ *     code too, and the outputs it concerns are NaN, status word or not.
  */
 
 /* q, k (optionally) normed and rotated, q to q_out, k and v appended to the

@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 #pragma unroll
     for (int e = 0; e < E; ++e) o[r][e] = 0.f;
   }
+  bool expired = false;
   for (int k = 0; k < mine; ++k) {
     const int j0 = w.sp.page(w.i0 + warp + DW * k) * PG;
     const bool gone = bad >> (k % 8) & 1;
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
       const long long t0 = clock64();  // the copies still under way end before their memory is used again
       while (clock64() - t0 < 1 << 20) {
       }
+      expired = true;
       break;
     }
     const KV* vp = reinterpret_cast<const KV*>(sm.ring[warp][(2 * k + 1) % S]) + lane * E;
@@ -411,7 +413,7 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
     for (int d = 4; d < 32; d *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
     if (lane == 0) {
       sm.join.m[warp][r] = m[r];
-      sm.join.l[warp][r] = l[r];
+      sm.join.l[warp][r] = expired ? NAN : l[r];  // NaN: so is every output that this is a part of
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sm.join.o[warp][r][lane * E + e] = o[r][e];
@@ -665,6 +667,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
 #pragma unroll
   for (int i = 0; i < NB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m = -INFINITY, l = 0.f;  // of head g; l of this lane's keys
+  bool expired = false;
   // The first terms' sums of whole runs of FOLD pages, in units of 2^kept_m: in registers, or, where the runs are long,
   // in local memory (asm: so that they take no registers from the loop) from the first whole run on.
   float kept_here[NB * 8 * 2], kept_m = -INFINITY;
@@ -692,6 +695,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
       const long long t0 = clock64();  // the copies still under way end before their memory is used again
       while (clock64() - t0 < 1 << 20) {
       }
+      expired = true;
       break;
     }
     const uint8_t* ks = slots + k % S * 2 * C::PAGE;
@@ -779,7 +783,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
   __syncthreads();  // the ring becomes the join's memory
   if (t == 0) {
     sm.join.m[warp][g] = m;
-    sm.join.l[warp][g] = l;
+    sm.join.l[warp][g] = expired ? NAN : l;  // NaN: so is every output that this is a part of
   }
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -794,7 +798,7 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
 #pragma unroll
     for (int i = 0; i < NB * 8; ++i) nan = nan || o[i][0] != o[i][0] || o[i][1] != o[i][1];
     // rows of one term of q: a sum of weights that is not finite is the formula's
-    unsigned again = __ballot_sync(0xffffffffu, nan && g < w.n_rows && (SPLIT || l < INFINITY));
+    unsigned again = __ballot_sync(0xffffffffu, nan && !expired && g < w.n_rows && (SPLIT || l < INFINITY));
     while (again) {
       const int r = (__ffs(again) - 1) / 4;
       again &= ~(0xfu << (4 * r));

@@ -886,6 +886,15 @@ __global__ void __launch_bounds__(TT, 1)
     while (clock64() - t0 < 1 << 20) {
     }
     __syncthreads();
+    // the CTA's rows are NaN: alone, or by their part's sum
+    if (parts > 1) {
+      for (int i = tid; i < C::ROWS; i += TT) ml[i] = make_float2(-INFINITY, NAN);
+    } else {
+      for (int i = tid; i < n_rows * HD; i += TT) {
+        const int r = t.row0 + i / HD;
+        store_elem(p.out, ((int64_t)(t.q0 + r / G) * p.n_head + hk * G + r % G) * HD + i % HD, NAN, p.io);
+      }
+    }
   }
   if (parts > 1) {
     // Each CTA adds the parts of its share of the rows, in order, each warp a run of rows; lane = (row, part) for the

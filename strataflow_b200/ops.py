@@ -131,10 +131,12 @@ def sample_logits(logits: torch.Tensor, temperature: float, top_k: int = 0, top_
 
 # ---- paged-cache operators (sfk_qk_norm_rope_append, sfk_attn_*_window) ---------
 # They run on the current stream of the tensors' device and return without
-# waiting; nothing is allocated but the output, so they can be captured into a
+# waiting; nothing is allocated but the output and, for single tokens over a long
+# context, a workspace (by torch, on that stream), so they can be captured into a
 # CUDA graph.  Refusals raise SfkError (invalid argument).  `status`, an int32
 # CUDA tensor of one zero, collects what only the device can see (a page id or a
-# position outside its range); check_status reads it.
+# position outside its range, a wait inside a kernel that ran out: the outputs
+# concerned are NaN then); check_status reads it.
 _ROW_TYPES = {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
 _KV_TYPES = {torch.float32: L.KV_F32, torch.float16: L.KV_F16, torch.bfloat16: L.KV_BF16}
 
