@@ -347,3 +347,68 @@ def test_append_in_place_of_a_packed_row(cuda, io, n):
             continue
         with pytest.raises(L.SfkError, match="overlaps"):
             run(x, bad)
+
+
+# ---- long contexts: what an elementwise bound cannot see ---------------------------------------------------
+@pytest.mark.parametrize("form,copies", FORMS)
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n", [20000, 9001])
+def test_decode_counts_every_key_once(cuda, form, copies, io, kv, hd, n):
+    """Equal weights (q = 0) and values that are 1 at one dim of each key: each dim is the share of its keys, about
+    n / hd of them.  A page lost or taken twice is 16 keys of dims of their own, 16 / (n / hd) or more of these.  Weights,
+    sums of whole numbers up to n and of weights are exact; one division and the output's rounding are left."""
+    c = Cache([n], 2, hd, kv, 11)
+    j = torch.arange(n, device="cuda")
+    c.values[0].copy_((j[:, None] // PG % hd == torch.arange(hd, device="cuda"))[:, None])
+    store(c)
+    q = torch.zeros((copies, 8, hd), dtype=io, device="cuda")
+    table, pos = c.table.expand(copies, -1).contiguous(), torch.full((copies,), n - 1, dtype=torch.int32, device="cuda")
+    got = decode_as(form, q, c, table, pos).double()
+    want = c.values[0][:, 0].double().mean(0).expand_as(got)
+    assert want.min() > 0
+    check(got, want, (2.0 ** -21 + half_step(io)) * want)
+
+
+@pytest.mark.parametrize("form,copies", FORMS)
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_decode_long_contexts_by_their_norm(cuda, form, copies, io, kv, hd):
+    """Random scores and values at 20000 keys.  Errors of the elements are independent: as a root of squares the scores'
+    rounding (hd + 6 steps of 2^-24 of a sum whose rms is 1: 2^-24 (hd + 6)^(1/2) < 2^-19), the exponential's 2^-22 and
+    n additions of 2^-24 of a partial sum, which is the output's size at the end and less before, 2^-24 n^(1/2) < 2^-16.
+    A 16-bit output adds at most half a step of itself.  A page of 1250 would be 2^-5."""
+    n = 20000
+    c = Cache([n], 2, hd, kv, 12)
+    q = torch.randn((copies, 8, hd), generator=gen(13), device="cuda").to(io)
+    table, pos = c.table.expand(copies, -1).contiguous(), torch.full((copies,), n - 1, dtype=torch.int32, device="cuda")
+    got = decode_as(form, q, c, table, pos)[:4].double()
+    want = reference(q[:4], c.keys[0], c.values[0], [n - 1] * min(4, copies), 0, 0)[0]
+    bound = 2.0 ** -16 + (half_step(io) if io != F32 else 0)
+    assert float((got - want).norm() / want.norm()) < bound
+    assert abs(float((got * want).sum() / (want * want).sum()) - 1) < bound
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window,n_sink", [(0, 0), (7003, 40)])
+@pytest.mark.parametrize("n_q", [3, 700])
+def test_windows_and_prompts_count_every_key_once(cuda, io, kv, hd, window, n_sink, n_q):
+    """The same for a window with sinks and for prompts, their keys split over CTAs or not.  A prompt's polynomial
+    exponential makes weights of a few columns 7.5e-5 (bf16) or 2.7e-6 (f16) smaller before they are rounded."""
+    n = 20000
+    c = Cache([n], 2, hd, kv, 11)
+    j = torch.arange(n, device="cuda")
+    c.values[0].copy_((j[:, None] // PG % hd == torch.arange(hd, device="cuda"))[:, None])
+    store(c)
+    q = torch.zeros((n_q, 8, hd), dtype=io, device="cuda")
+    p = torch.arange(n - n_q, n, device="cuda")[:, None]
+    seen = j <= p
+    if window:
+        seen &= (j > p - window) | (j < n_sink)
+    want = (seen.double() @ c.values[0][:, 0].double() / seen.sum(-1, keepdim=True))[:, None]
+    tol = (2.0 ** -21 + (half_step(io) if io != F32 else 0)) * want
+    check(decode(q[-1:], c, window=window, n_sink=n_sink), want[-1:], tol[-1:])
+    if io != F32:
+        tol = tol + (7.5e-5 if kv == BF16 else 2.7e-6) * want
+    check(prefill(q, c, n - n_q, window=window, n_sink=n_sink), want, tol)
