@@ -98,6 +98,18 @@ inline cudaError_t allow_smem(size_t bytes) {
 }
 
 #ifdef __CUDACC__
+// A launch and its own status: cudaGetLastError after it would also return what an earlier call of another kind left
+// behind (an engine that did not fit the card).
+template <class P>
+inline cudaError_t launch_own(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t st, const P& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 // ---- element access -----------------------------------------------------------
 template <class T>
 __device__ __forceinline__ float to_f32(T x);

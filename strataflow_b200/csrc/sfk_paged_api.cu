@@ -27,6 +27,7 @@ sfk_status pfail(sfk_status st, const char* fmt, ...) {
 }
 sfk_status cuda_result(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return SFK_OK;
+  cudaGetLastError();  // reported here, and to no later call
   return pfail(e == cudaErrorMemoryAllocation ? SFK_ERR_OUT_OF_MEMORY : SFK_ERR_RUNTIME, "%s: %s", what,
                cudaGetErrorString(e));
 }

@@ -218,14 +218,15 @@ cudaError_t launch_t(AppendParams& p, int sm_count, cudaStream_t st) {
   p.share = (int)(wave < 1 ? 1 : wave < (steps + 1) / 2 ? wave : (steps + 1) / 2);
   const int64_t ctas = ((int64_t)p.n_tok * p.share + AW - 1) / AW;
   const size_t smem = (size_t)AW * (p.q_norm == p.k_norm ? 1 : 2) * p.hd * sizeof(float2);
-  const dim3 grid((unsigned)ctas), block(AW * 32);
-  if (p.hd == 64) append_kernel<IO, KV, 8, true><<<grid, block, smem, st>>>(p);
-  else if (p.hd == 128) append_kernel<IO, KV, 16, true><<<grid, block, smem, st>>>(p);
-  else if (lpr == 4) append_kernel<IO, KV, 4, false><<<grid, block, smem, st>>>(p);
-  else if (lpr == 8) append_kernel<IO, KV, 8, false><<<grid, block, smem, st>>>(p);
-  else if (lpr == 16) append_kernel<IO, KV, 16, false><<<grid, block, smem, st>>>(p);
-  else append_kernel<IO, KV, 32, false><<<grid, block, smem, st>>>(p);
-  return cudaGetLastError();
+  auto launch = [&](void (*kernel)(AppendParams)) {
+    return launch_own(kernel, dim3((unsigned)ctas), AW * 32, smem, st, p);
+  };
+  if (p.hd == 64) return launch(append_kernel<IO, KV, 8, true>);
+  if (p.hd == 128) return launch(append_kernel<IO, KV, 16, true>);
+  if (lpr == 4) return launch(append_kernel<IO, KV, 4, false>);
+  if (lpr == 8) return launch(append_kernel<IO, KV, 8, false>);
+  if (lpr == 16) return launch(append_kernel<IO, KV, 16, false>);
+  return launch(append_kernel<IO, KV, 32, false>);
 }
 
 template <class IO>

@@ -223,8 +223,7 @@ cudaError_t launch_fma(WindowAttnParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int64_t group = p.n_head / p.n_head_kv;
   const dim3 grid((unsigned)(p.n_tok * group / FR + p.n_seq), (unsigned)p.n_head_kv);
-  prefill_fma_kernel<KV, HD><<<grid, FT, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_own(prefill_fma_kernel<KV, HD>, grid, FT, smem, st, p);
 }
 
 template <class KV>

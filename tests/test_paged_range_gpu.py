@@ -412,3 +412,23 @@ def test_windows_and_prompts_count_every_key_once(cuda, io, kv, hd, window, n_si
     if io != F32:
         tol = tol + (7.5e-5 if kv == BF16 else 2.7e-6) * want
     check(prefill(q, c, n - n_q, window=window, n_sink=n_sink), want, tol)
+
+
+# ---- an error of another call -------------------------------------------------------------------------------
+@pytest.mark.parametrize("io,kv", [(F32, F32), (BF16, BF16)])
+def test_an_earlier_error_is_not_reported_again(cuda, io, kv):
+    """An engine larger than the card fails to allocate; the operators' calls after it are fine."""
+    from strataflow_b200 import engine as E
+    from strataflow_b200 import lib as L
+    from strataflow_b200 import ops
+    c = Cache([20], 2, 64, kv, 1)
+    q = torch.randn((20, 4, 64), generator=gen(2), device="cuda").to(io)
+    k = torch.randn((20, 2, 64), generator=gen(3), device="cuda").to(io)
+    pos, freqs = torch.arange(20, dtype=torch.int32, device="cuda"), ops.rope_freqs(64)
+    calls = (lambda: ops.qk_norm_rope_append(q, k, k, c.k, c.v, c.table, pos, seq=torch.zeros_like(pos), freqs=freqs),
+             lambda: prefill(q, c, 0), lambda: decode(q[:1], c))
+    for f in calls:
+        want = f()
+        with pytest.raises(L.SfkError):
+            E.Engine(E.tiny_config(n_vocab=800_000_000))
+        assert torch.equal(f(), want)
