@@ -271,6 +271,26 @@ __device__ __forceinline__ bool key_seen(int j, int p, int window, int n_sink) {
   return j <= p && (window == 0 || j > p - window || j < n_sink);
 }
 
+// Where q_start descends: bits of the lane's four starts that lie below one before them, in this lane, in the lanes
+// before it or (top) in an earlier step, and the largest start so far.  Out of line, it is never called for a q_start
+// that ascends.
+static __device__ __noinline__ int2 begin_below(int a0, int a1, int a2, int a3, int top) {
+  const int lane = threadIdx.x & 31, a[4] = {a0, a1, a2, a3};
+  int upto = max(max(a0, a1), max(a2, a3));  // of this lane and those before it
+  for (int d = 1; d < 32; d *= 2) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto = max(upto, v);
+  }
+  int before = __shfl_up_sync(0xffffffffu, upto, 1);
+  before = lane ? max(before, top) : top;
+  unsigned below = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (a[i] < before) below |= 1u << i;
+    before = max(before, a[i]);
+  }
+  return make_int2((int)below, max(top, __shfl_sync(0xffffffffu, upto, 31)));
+}
+
 // Tile `idx` of the ragged batch: tiles of RT rows, sequence by sequence, the
 // last tile of a sequence first (its rows see the most keys).  All lanes of
 // the warp call it and get the same answer; seq = -1 past the last tile.
@@ -284,6 +304,8 @@ __device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx
   const int64_t group = p.n_head / p.n_head_kv;
   Tile t;
   t.seq = -1;
+  bool descends = false;  // q_start went back: what begins below a start before it shares rows, and counts as bad
+  int top = 0;            // then: the largest start so far
   for (int s0 = 0; s0 < p.n_seq; s0 += 32 * V) {
     const int s = s0 + lane * V;
     int at[V + 1], len[V], n[V];
@@ -292,11 +314,21 @@ __device__ __forceinline__ Tile find_tile(const WindowAttnParams& p, int64_t idx
     for (int i = 0; i <= V; ++i) at[i] = s + i <= p.n_seq ? p.q_start[s + i] : 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) len[i] = s + i < p.n_seq ? p.kv_len[s + i] : 0;
+    unsigned below = 0;  // bit i: begins below a start before it
+    bool back = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) back = back || (s + i < p.n_seq && at[i + 1] < at[i]);
+    descends = __any_sync(0xffffffffu, back) || descends;
+    if (descends) {
+      const int2 r = begin_below(at[0], at[1], at[2], at[3], top);
+      below = r.x;
+      top = r.y;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       n[i] = 0;
       if (s + i < p.n_seq) {
-        if (at[i] < 0 || at[i + 1] < at[i] || at[i + 1] > p.n_tok || len[i] < 0 || (len[i] + (int64_t)PG - 1) / PG > p.max_pages)
+        if (at[i] < 0 || (below >> i & 1) || at[i + 1] < at[i] || at[i + 1] > p.n_tok || len[i] < 0 || (len[i] + (int64_t)PG - 1) / PG > p.max_pages)
           report(p.status, ERR_BAD_POS);  // nothing of this sequence is read or written
         else
           n[i] = at[i + 1] - at[i];

@@ -432,3 +432,29 @@ def test_an_earlier_error_is_not_reported_again(cuda, io, kv):
         with pytest.raises(L.SfkError):
             E.Engine(E.tiny_config(n_vocab=800_000_000))
         assert torch.equal(f(), want)
+
+
+# ---- sequences whose rows overlap ---------------------------------------------------------------------------
+@pytest.mark.parametrize("io,kv,hd", [(F32, F32, 64), (F32, F16, 128), (BF16, BF16, 128)])
+@pytest.mark.parametrize("first,late", [(0, 2), (3, 6), (125, 127), (126, 128), (127, 129), (60, 140)])
+def test_prefill_q_start_that_descends_leaves_the_other_sequences_alone(cuda, io, kv, hd, first, late):
+    """q_start goes back once, into the rows of sequence `first`: the sequence that ends there and the one that begins
+    there are reported and touch nothing, all others are as they were."""
+    from strataflow_b200 import lib as L
+    from strataflow_b200 import ops
+    n_seq, each = 150, 20
+    c = Cache([each] * n_seq, 1, hd, kv, 1)
+    q = torch.randn((n_seq * each, 2, hd), generator=gen(2), device="cuda").to(io)
+    start = torch.arange(n_seq + 1, dtype=torch.int32, device="cuda") * each
+    kv_len = torch.full((n_seq,), each, dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    good = ops.attn_prefill_window(q, c.k, c.v, c.table, start, kv_len, status=status)
+    ops.check_status(status)
+    start[late] = first * each + 10
+    out = torch.full_like(good, 5.0)
+    ops.attn_prefill_window(q, c.k, c.v, c.table, start, kv_len, out=out, status=status)
+    with pytest.raises(L.SfkError, match="position or length"):
+        ops.check_status(status)
+    a, b = (late - 1) * each, (late + 1) * each
+    assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])
+    assert (out[a:b] == 5.0).all()
