@@ -458,3 +458,30 @@ def test_prefill_q_start_that_descends_leaves_the_other_sequences_alone(cuda, io
     a, b = (late - 1) * each, (late + 1) * each
     assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])
     assert (out[a:b] == 5.0).all()
+
+
+# ---- queries at the ends of f32 -----------------------------------------------------------------------------
+@pytest.mark.parametrize("kv", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("n", [40, 700])
+def test_tiny_and_huge_queries(cuda, kv, hd, n):
+    """q near 2^-126 under a small scale: scores of 0, the mean of the values.  q near 2^127 under a scale above 1, keys
+    of at most 2^-2: scores up to 2^127 and the others 2^100 below, the largest key's value alone."""
+    c = Cache([n], 2, hd, kv, 1)
+    g = gen(2)
+    v = c.values[0].double().repeat_interleave(2, 1)
+    q = torch.randn((1, 4, hd), generator=g, device="cuda") * 1e-37
+    want = v.mean(0, keepdim=True)
+    for got in (decode(q, c, scale=1e-9), prefill(q, c, n - 1, scale=1e-9)):
+        check(got, want, (n + 16) * 2.0 ** -23 * v.abs().amax().expand_as(want))
+    top = n // 3
+    scores = torch.arange(n, device="cuda").float() / n * 2.0 ** -4
+    scores[top] = 2.0 ** -2
+    c.keys[0].zero_()
+    c.keys[0][..., 0] = scores.to(kv)[:, None]
+    store(c)
+    q.zero_()
+    q[..., 0] = 2.0 ** 126
+    want = v[top][None]
+    for got in (decode(q, c, scale=4.0), prefill(q, c, n - 1, scale=4.0)):
+        check(got, want, 2.0 ** -20 * want.abs())
