@@ -58,6 +58,8 @@ sfk_status fail(sfk_status st, const char* fmt, ...) {
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
   g_err = buf;
+  // reported here, and to no later call: launches read the runtime's last error
+  if (st == SFK_ERR_RUNTIME || st == SFK_ERR_OUT_OF_MEMORY) cudaGetLastError();
   return st;
 }
 

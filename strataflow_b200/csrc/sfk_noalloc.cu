@@ -43,6 +43,7 @@ sfk_status nfail(sfk_status st, const char* fmt, ...) {
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
   sfk::set_last_error(buf);  // what sfk_last_error() returns on this thread
+  if (st == SFK_ERR_RUNTIME) cudaGetLastError();  // reported here, and to no later call
   return st;
 }
 
