@@ -443,11 +443,13 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 // a finite value stays finite under it, as under the softmax's own weights.
 // The product's f32 sum drops what falls below its last bits, each time, towards 0: of
 // values of one sign 2.1e-4 was gone after the 2048 pages that a warp of a full batch takes
-// at 131072 keys.  So O of FOLD pages is a sum of its own, added to the kept one by f32
-// additions that round to nearest: 8 pages for 32-bit rows (4e-7 of the result, as prompts
-// have it), 512 for f16 rows (5e-5, a tenth of f16's half step).  bf16 rows keep one sum: those
-// 2.1e-4 are a twentieth of their half step, and runs of 512 pages took 673 us where one sum
-// takes 667 (eight long sequences; 32-bit rows, one sequence of 32768: 32.8, 32.0 without).
+// at 131072 keys.  So a warp of many pages (RUNS) sums O in runs, which it adds to a kept O by
+// f32 additions that round to nearest: runs of 8 pages for 32-bit rows (4e-7 of the result, as
+// prompts have it), of 512 for f16 rows (5e-5, a tenth of f16's half step).  A warp of at
+// most 12 pages of 32-bit rows (8e-7), or of 512, does without: one sequence of 32768, 32-bit
+// rows: 30.0 us, 31.3 with runs.  bf16 rows keep one sum: those 2.1e-4 are a twentieth of
+// their half step, and runs of 512 pages took 673 us where one sum takes 667 (eight long
+// sequences).
 // Eight sequences of 131072 keys, 64 heads of 128 over 8, bf16: 645 us, 6.66 TB/s, what a
 // copy reaches (operands straight from global memory: 1190 us).  One sequence of
 // 32768, f32 rows over f16: 29.8 us, of which 20.5 are the bytes and the rest the chain
@@ -556,7 +558,13 @@ struct MmaSmem {
   uint64_t full[DW][C::STAGES];
 };
 
-template <class KV, int HD, bool SPLIT, int DW>
+// Pages of a run, and the most that a warp may take without runs.
+template <bool SPLIT>
+constexpr int RUN = SPLIT ? 8 : 512;
+template <bool SPLIT>
+constexpr int MAX_RUN = SPLIT ? 12 : 512;
+
+template <class KV, int HD, bool SPLIT, int DW, bool RUNS>
 __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
     decode_mma_kernel(const __grid_constant__ WindowAttnParams p, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap) {
@@ -564,7 +572,6 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
   using C = MmaCfg<HD, DW>;
   using Smem = MmaSmem<HD, DW>;
   constexpr int DT = DW * 32, NB = C::HDP / 64, S = C::STAGES;
-  constexpr int FOLD = SPLIT ? 8 : 512;  // pages (bf16: all)
   constexpr float RAISE = 4.f, BIAS = BF16 ? -RAISE : 11.f;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -668,14 +675,14 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
   for (int i = 0; i < NB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m = -INFINITY, l = 0.f;  // of head g; l of this lane's keys
   bool expired = false;
-  // The first terms' sums of whole runs of FOLD pages, in units of 2^kept_m: in registers, or, where the runs are long,
+  // The first terms' sums of whole runs, in units of 2^kept_m: in registers, or, where the runs are long,
   // in local memory (asm: so that they take no registers from the loop) from the first whole run on.
   float kept_here[NB * 8 * 2], kept_m = -INFINITY;
   float* kept = kept_here;
-  if constexpr (SPLIT) {
+  if constexpr (RUNS && SPLIT) {
 #pragma unroll
     for (int i = 0; i < NB * 8 * 2; ++i) kept[i] = 0.f;
-  } else if constexpr (!BF16) {
+  } else if constexpr (RUNS) {
     asm volatile("" : "+l"(kept)::"memory");
   }
   auto fold = [&](bool any) {  // any: there are kept sums
@@ -769,9 +776,9 @@ __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
     }
     __syncwarp();  // every lane is done with the slot
     if (k + S < mine) issue_noting(k + S);
-    if (!BF16 && k % FOLD == FOLD - 1) fold(k >= FOLD);
+    if (RUNS && k % RUN<SPLIT> == RUN<SPLIT> - 1) fold(k >= RUN<SPLIT>);
   }
-  if (SPLIT || (!BF16 && mine >= FOLD)) {
+  if (RUNS && (SPLIT || mine >= RUN<SPLIT>)) {
     const float f = kept_m == -INFINITY ? 0.f : exp2_approx(kept_m - m);
 #pragma unroll
     for (int i = 0; i < NB * 8; ++i)
@@ -906,8 +913,13 @@ cudaError_t launch_mma(WindowAttnParams& p, int kv, int sm_count, cudaStream_t s
   if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, (HD + 63) / 64);
   if (e != cudaSuccess) return e;
   pick_parts(p, HD <= 128 ? 3 : 1, HD, sm_count);
-  return launch_parts<decode_mma_kernel<KV, HD, SPLIT, DEC_W>>(p, row_tiles(p), DEC_W * 32, sizeof(Smem) + 1024, st, km,
-                                                               vm);
+  const auto launch = [&](auto runs) {
+    return launch_parts<decode_mma_kernel<KV, HD, SPLIT, DEC_W, decltype(runs)::value>>(p, row_tiles(p), DEC_W * 32,
+                                                                                       sizeof(Smem) + 1024, st, km, vm);
+  };
+  if constexpr (std::is_same<KV, __half>::value)
+    if (max_seen_pages(p) > (int64_t)p.parts * DEC_W * MAX_RUN<SPLIT>) return launch(std::true_type());
+  return launch(std::false_type());
 }
 template <class KV, int HD>
 cudaError_t launch_16(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {

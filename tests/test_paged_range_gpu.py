@@ -188,6 +188,20 @@ def test_decode_of_16_bit_rows_has_no_drift(cuda, form, copies, kv, hd):
     assert float((got - want).norm() / want.norm()) < half_step(kv)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("pages", [8, 12, 13, 16, 17])
+def test_decode_of_32_bit_rows_has_no_drift_at_short_chains(cuda, hd, pages):
+    """32 warps of a cluster take `pages` pages each of values of one sign: 2^-20, as at long contexts."""
+    n = pages * 32 * PG
+    c = Cache([n], 1, hd, F16, 14)
+    c.values[0].copy_(0.5 + torch.rand((n, 1, hd), generator=gen(15), device="cuda"))
+    store(c)
+    q = torch.randn((1, 4, hd), generator=gen(16), device="cuda") * 0.25
+    got = decode_as("cluster", q, c, c.table, torch.full((1,), n - 1, dtype=torch.int32, device="cuda")).double()
+    want = reference(q, c.keys[0], c.values[0], [n - 1], 0, 0)[0]
+    assert abs(float((got * want).sum() / (want * want).sum()) - 1) < 2.0 ** -20
+
+
 @pytest.mark.parametrize("kv", [F16, BF16])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("n_q", [3, 2400])
