@@ -4,11 +4,11 @@
 //
 //   s_j = scale q . k_j  for the seen keys j;  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
 //
-// Bound by memory: each seen key and value is read once for all query heads
-// of its kv head.  The seen pages of one (sequence, kv head, 8 query heads) are
-// split over CTAs; each warp takes every W-th page of its CTA's run with a
-// running maximum, sum and output of its own (f32).  The partials of the warps
-// meet in shared memory, those of the CTAs
+// Bound by memory: each seen key and value is read once for 8 query heads of its
+// kv head (of more, every 8 read it again).  The seen pages of one (sequence, kv
+// head, 8 query heads) are split over CTAs; each warp takes every W-th page of its
+// CTA's run with a running maximum, sum and output of its own (f32).  The partials
+// of the warps meet in shared memory, those of the CTAs
 //   - in the distributed shared memory of a cluster of up to 8 (no scratch, one
 //     launch), or,
 //   - where the batch is too small for such clusters to fill the GPU, in the
@@ -223,8 +223,12 @@ __device__ __forceinline__ int page_id(const WindowAttnParams& p, const Work& w,
 // V, ...).  Scores: lane (g, t) multiplies four dims of every 16 of keys g and g + 8
 // by the query rows in shared memory; odd g take the two halves of 32 dims in the
 // other order, so that two keys' rows never meet in a bank.  Values: the lane owns
-// HD / 32 output dims.  64 multiply-adds to 10 shared loads, and 64 bytes of cache a
-// cycle at the multiply-add rate, above what memory delivers.
+// HD / 32 output dims.  64 multiply-adds to 10 shared loads.
+// Sixteen sequences of 4096 keys, 32 heads of 128 over 8, f32: 133 us, 4.0 TB/s; a bf16
+// cache of half the bytes 129 us.  So memory is not what binds it: the ring leaves room
+// for two CTAs to an SM, two warps to a scheduler, which wait for shared loads and fixed
+// latencies half of the time (issue slots 0.47 busy), 8 query rows are computed where four
+// heads need 4, and 256 CTAs on 296 places leave a seventh of them empty.
 template <class KV, int HD>
 struct CcCfg {
   static constexpr int R = 8, DW = 4;
@@ -452,7 +456,7 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 // sequences).
 // Eight sequences of 131072 keys, 64 heads of 128 over 8, bf16: 645 us, 6.66 TB/s, what a
 // copy reaches (operands straight from global memory: 1190 us).  One sequence of
-// 32768, f32 rows over f16: 29.8 us, of which 20.5 are the bytes and the rest the chain
+// 32768, f32 rows over f16: 30.0 us, of which 20.5 are the bytes and the rest the chain
 // before the first page and behind the last one.  Three CTAs of two slots a warp,
 // not two of three: 38 and 49 us for 48 ragged windows of 1024, 645 and 647 for the
 // eight long ones.
