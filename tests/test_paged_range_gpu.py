@@ -46,7 +46,7 @@ def decode(q, c, **kw):
 
 # ---- a dominant key over a long tail ---------------------------------------------------------------------
 @pytest.mark.parametrize("io,kv", TYPES)
-@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
 @pytest.mark.parametrize("n_q,hq", [(3, 4), (2400, 8)])
 def test_prefill_dominant_key_of_zero_value(cuda, io, kv, hd, n_q, hq):
     """One key 18 nats above 30000 others, its value 0, the others' of one sign: the output is the tail alone, of which
@@ -223,6 +223,25 @@ def test_prefill_of_16_bit_rows_has_no_drift(cuda, kv, hd, n_q):
         assert float((got[i:i + 1].double() - want).norm() / want.norm()) < half_step(kv)
 
 
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("hd", [32, 128])
+@pytest.mark.parametrize("n_q,hq", [(3, 4), (2400, 8)])
+def test_prefill_through_a_long_window(cuda, kv, hd, n_q, hq):
+    """A window of 25000 of 32000 keys behind 100 sinks, scores that rise along the context so that the maximum moves in
+    every run of keys, values of both signs: by the norm, half a step for the output, half a step and the polynomial for
+    the weights."""
+    n, window, n_sink = 32000, 25000, 100
+    scores = torch.arange(n, device="cuda") / n * 12 + 0.5 * torch.randn(n, generator=gen(1), device="cuda")
+    q, c = one_number(n, hq, 1, hd, kv, kv, scores, 3)
+    q = q.expand(n_q, -1, -1).contiguous()
+    got = prefill(q, c, n - n_q, scale=0.125, window=window, n_sink=n_sink).double()
+    for i in (0, n_q // 2, n_q - 1):
+        want, _, absv = reference(q[i:i + 1], c.keys[0], c.values[0], [n - n_q + i], window, n_sink, 0.125)
+        bound = half_step(kv) * want.norm() + (half_step(kv) + 1.5e-4) * absv.norm()
+        assert float((got[i:i + 1] - want).norm()) < float(bound)
+        assert torch.equal(got[i], got[i][:1].expand_as(got[i]))  # every head has the same scores
+
+
 # ---- no weight at all ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("io,kv", TYPES)
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
@@ -366,7 +385,7 @@ def test_append_in_place_of_a_packed_row(cuda, io, n):
 # ---- long contexts: what an elementwise bound cannot see ---------------------------------------------------
 @pytest.mark.parametrize("form,copies", FORMS)
 @pytest.mark.parametrize("io,kv", TYPES)
-@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
 @pytest.mark.parametrize("n", [20000, 9001])
 def test_decode_counts_every_key_once(cuda, form, copies, io, kv, hd, n):
     """Equal weights (q = 0) and values that are 1 at one dim of each key: each dim is the share of its keys, about
