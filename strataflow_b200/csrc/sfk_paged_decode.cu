@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(CcCfg<KV, HD>::DW * 32) decode_cc_kernel(const
 // f32 additions that round to nearest: runs of 8 pages for 32-bit rows (4e-7 of the result, as
 // prompts have it), of 512 for f16 rows (5e-5, a tenth of f16's half step).  A warp of at
 // most 12 pages of 32-bit rows (8e-7), or of 512, does without: one sequence of 32768, 32-bit
-// rows: 30.0 us, 31.3 with runs.  bf16 rows keep one sum: those 2.1e-4 are a twentieth of
-// their half step, and runs of 512 pages took 673 us where one sum takes 667 (eight long
+// rows: 30.0 us, 31.3 with runs.  bf16 rows do without up to 2048 pages: those 2.1e-4 are a
+// twentieth of their half step, and runs took 673 us where one sum takes 667 (eight long
 // sequences).
 // Eight sequences of 131072 keys, 64 heads of 128 over 8, bf16: 645 us, 6.66 TB/s, what a
 // copy reaches (operands straight from global memory: 1190 us).  One sequence of
@@ -565,8 +565,8 @@ struct MmaSmem {
 // Pages of a run, and the most that a warp may take without runs.
 template <bool SPLIT>
 constexpr int RUN = SPLIT ? 8 : 512;
-template <bool SPLIT>
-constexpr int MAX_RUN = SPLIT ? 12 : 512;
+template <bool SPLIT, bool BF16>
+constexpr int MAX_RUN = SPLIT ? 12 : BF16 ? 2048 : 512;
 
 template <class KV, int HD, bool SPLIT, int DW, bool RUNS>
 __global__ void __launch_bounds__(DW * 32, HD <= 128 ? 3 : 1)
@@ -921,9 +921,8 @@ cudaError_t launch_mma(WindowAttnParams& p, int kv, int sm_count, cudaStream_t s
     return launch_parts<decode_mma_kernel<KV, HD, SPLIT, DEC_W, decltype(runs)::value>>(p, row_tiles(p), DEC_W * 32,
                                                                                        sizeof(Smem) + 1024, st, km, vm);
   };
-  if constexpr (std::is_same<KV, __half>::value)
-    if (max_seen_pages(p) > (int64_t)p.parts * DEC_W * MAX_RUN<SPLIT>) return launch(std::true_type());
-  return launch(std::false_type());
+  constexpr int most = MAX_RUN<SPLIT, std::is_same<KV, __nv_bfloat16>::value>;
+  return max_seen_pages(p) > (int64_t)p.parts * DEC_W * most ? launch(std::true_type()) : launch(std::false_type());
 }
 template <class KV, int HD>
 cudaError_t launch_16(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st) {

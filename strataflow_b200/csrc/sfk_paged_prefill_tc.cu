@@ -45,8 +45,9 @@
 // 0: 8.3e-4 of values of one sign were gone after 131072 keys, more than half a step of
 // f16.  So f16 rows start O anew every 10240 keys and keep the sum in local memory, added
 // to the nearest (6.7e-5; 2048 tokens at 30000 keys, 32 heads of 128: 875 us with and
-// without, heads of 64: 858 and 832).  bf16 rows keep one accumulator: those 8.3e-4 are a
-// fifth of their half step, and a second loop around the tiles took 2 % there.
+// without, heads of 64: 858 and 832).  bf16 rows do so every 81920 keys where a CTA may
+// walk more than 131072: up to there one accumulator loses a fifth of their half step, and
+// the second loop around the tiles takes 2 %.
 //
 // 32-bit rows over an f16 cache (SPLIT): q, scaled by a power of two per row,
 // is the sum of two f16 numbers and so is each P (22 bits), and each product
@@ -106,6 +107,12 @@ struct Cfg {
   static constexpr int P0 = TILES * TK, PCOLS = TK / 2 * NS, O0 = 512 - OBUF * HDP;
   static_assert(P0 + TILES * PCOLS <= O0 && STAGES >= 2 && TK % PG == 0, "tile sizes");
 };
+
+// Keys that meet in one accumulator of 16-bit rows, and how many may without a kernel of RUNS
+template <class KV>
+constexpr int RUN_KEYS = std::is_same<KV, __nv_bfloat16>::value ? 81920 : 10240;
+template <class KV>
+constexpr int64_t MAX_RUN_KEYS = std::is_same<KV, __nv_bfloat16>::value ? 131072 : 0;
 
 struct Ctl {
   uint64_t full[2][4], empty[2][4];  // [K, V][stage]
@@ -331,15 +338,14 @@ __device__ __noinline__ void recompute_row(const WindowAttnParams& p, const Tile
 }
 
 // ---- the kernel ----------------------------------------------------------------------------
-template <class KV, int HD, bool SPLIT>
+template <class KV, int HD, bool SPLIT, bool RUNS>  // RUNS: O is the sum of several accumulators
 __global__ void __launch_bounds__(TT, 1)
     prefill_tc_kernel(const __grid_constant__ WindowAttnParams p, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<HD, SPLIT>;
   constexpr bool BF16 = std::is_same<KV, __nv_bfloat16>::value;
   constexpr int HDP = C::HDP, NS = C::NS, TK = C::TK, PPT = C::PPT;
-  constexpr bool RUNS = !SPLIT && !BF16;               // O is the sum of several accumulators
-  constexpr int RUN = RUNS ? 128 * 80 / TK : 1 << 30;  // key tiles of one
+  constexpr int RUN = RUNS ? RUN_KEYS<KV> / TK : 1 << 30;  // key tiles of one
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = base;                   // [tile][term][half][128 rows][128 B]
@@ -970,8 +976,6 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st)
   cudaError_t e = pool_map(&km, p.k_pages, kv, HD, rows, 1);
   if (e == cudaSuccess) e = pool_map(&vm, p.v_pages, kv, HD, rows, 1);
   if (e != cudaSuccess) return e;
-  e = allow_smem<prefill_tc_kernel<KV, HD, SPLIT>>(C::SMEM);
-  if (e != cudaSuccess) return e;
   // Few row tiles: their keys are split over clusters of 2, 4 or 8, as long as all clusters fit the GPU at a time
   // (clusters of 8 with one CTA to an SM: 15 of them were seen to fit 148 SMs) and a CTA keeps four key tiles; row
   // tiles of 128 then, if that still leaves half of the SMs without work.
@@ -1000,7 +1004,15 @@ cudaError_t launch_t(WindowAttnParams& p, int kv, int sm_count, cudaStream_t st)
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, prefill_tc_kernel<KV, HD, SPLIT>, p, km, vm);
+  const auto launch = [&](auto runs) {
+    constexpr auto kernel = prefill_tc_kernel<KV, HD, SPLIT, decltype(runs)::value>;
+    const cudaError_t e = allow_smem<kernel>(C::SMEM);
+    return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p, km, vm) : e;
+  };
+  if constexpr (!SPLIT)
+    if (pages * PG > p.key_parts * MAX_RUN_KEYS<KV>) return launch(std::true_type());
+  if constexpr (SPLIT || MAX_RUN_KEYS<KV> > 0) return launch(std::false_type());
+  return cudaErrorInvalidValue;  // f16 rows: a table has a page or more
 }
 
 template <class KV, bool SPLIT>

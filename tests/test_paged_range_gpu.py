@@ -242,6 +242,26 @@ def test_prefill_through_a_long_window(cuda, kv, hd, n_q, hq):
         assert torch.equal(got[i], got[i][:1].expand_as(got[i]))  # every head has the same scores
 
 
+@pytest.mark.parametrize("kv", [F16, BF16])
+def test_a_million_keys_of_one_sign(cuda, kv):
+    """What sums lose does not grow with the context: the bounds of 131072 keys at eight times as many, for single
+    tokens of a batch that gives each sequence one CTA and for prompts whose keys are not split."""
+    n, hd = 1 << 20, 64
+    c = Cache([n], 1, hd, kv, 14, poison=False)
+    scales = 2.0 ** (torch.arange(hd, device="cuda") / hd)
+    c.values[0].copy_((0.5 + torch.rand((n, 1, hd), generator=gen(15), device="cuda")) * scales)
+    store(c)
+    q = (torch.randn((2400, 8, hd), generator=gen(16), device="cuda") * 0.25).to(kv)
+    table, pos = c.table.expand(600, -1).contiguous(), torch.full((600,), n - 1, dtype=torch.int32, device="cuda")
+    one = decode_as("many", q[-600:], c, table, pos)[-1:].double()
+    all_ = prefill(q, c, n - 2400)[-1:].double()
+    want = reference(q[-1:], c.keys[0], c.values[0], [n - 1], 0, 0)[0]
+    for got, bound in ((one, 0.25), (all_, 0.41)):
+        gain = float((got * want).sum() / (want * want).sum()) - 1
+        assert abs(gain) < bound * half_step(kv), gain
+        assert float((got - want).norm() / want.norm()) < half_step(kv)
+
+
 # ---- no weight at all ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("io,kv", TYPES)
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
