@@ -321,7 +321,8 @@ def attn_decode_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
                        out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """sfk_attn_decode_window: q [n_seq][Hq][hd], one token of each sequence at
     positions[t] (negative: padding, zeros) over the keys it sees: j <= p and,
-    with window > 0, j > p - window or j < n_sink.  Returns [n_seq][Hq * hd]."""
+    with window > 0, j > p - window or j < n_sink.  Returns [n_seq][Hq * hd]
+    (`out`, which may be q's own memory where q is contiguous)."""
     dev = _cuda_device(q, "q")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -349,7 +350,8 @@ def attn_prefill_window(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     """sfk_attn_prefill_window: rows q_start[s] .. q_start[s+1]-1 of q
     [tokens][Hq][hd] are the newest of the kv_len[s] tokens of sequence s in
     the cache; each attends over the keys it sees (attn_decode_window).
-    Returns [tokens][Hq * hd]; rows of no sequence are not written."""
+    Returns [tokens][Hq * hd] (`out`, apart from q); rows of no sequence are
+    not written."""
     dev = _cuda_device(q, "q")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
